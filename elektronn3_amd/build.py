@@ -19,9 +19,12 @@ SOURCES = ['conv_mfma.hip', 'conv_v3.hip', 'conv_wino.hip', 'conv_wino4.hip', 'c
 # the 16-bit path is compiled a second time for IEEE half (-DE3_F16, external symbols renamed by f16_names.h; see csrc/bf16.h)
 F16_SOURCES = ['bf16_conv.hip', 'bf16_wgrad.hip', 'bf16_upconv.hip', 'bf16_ew.hip', 'bf16_first.hip', 'api_bf16.cpp', 'unet_bf16.cpp']
 HEADERS = ['common.h', 'kernels.h', 'brick_order.h', 'bf16.h', 'f16_names.h', 'plan_internal.h', os.path.join('..', '..', 'include', 'e3unet.h')]
-FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-Wall', '-Wno-unused-function', '-x', 'hip'] + os.environ.get('E3_HIPCC_EXTRA', '').split()
-# per-file extras.  wgrad_wino: the SLP vectoriser turns its scalar transforms into v_pk_* ops plus ~200 v_mov per brick
-# to pair the operands up; packed fp32 is not faster than two scalar ops on gfx950 (7 vs 2 x 4.5 cycles), the moves are pure loss.
+# No packed fp32 instructions (v_pk_add / mul / fma_f32), which hipcc -O3 forms from ordinary float code: some of their forms give wrong results on MI355X
+# now and then, without an error.  (The host pass warns that it does not know the feature.)  What they were worth, same box: fp32 training step 11.02 -> 11.65 ms,
+# Predictor tile 6.36 -> 6.87 ms; 16-bit step unchanged.
+NO_PACKED_F32 = ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
+FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-Wall', '-Wno-unused-function', '-x', 'hip'] + NO_PACKED_F32 + os.environ.get('E3_HIPCC_EXTRA', '').split()
+# per-file extras.  wgrad_wino: the SLP vectoriser pairs its scalar transforms up, which costs ~200 v_mov per brick.
 EXTRA_FLAGS = {'wgrad_wino.hip': ['-fno-slp-vectorize'], 'wgrad_wino2d.hip': ['-fno-slp-vectorize']}
 
 
@@ -61,7 +64,7 @@ def _build_locked(srcs, hdrs, force, verbose):
     def compile_one(job):
         src, f16 = job
         obj = os.path.join(OBJDIR, os.path.basename(src) + ('.f16.o' if f16 else '.o'))
-        if force or _stale(obj, [src] + hdrs):
+        if force or _stale(obj, [src] + hdrs + [os.path.abspath(__file__)]):      # (this file: the flags)
             extra = ['-DE3_F16', '-include', os.path.join(CSRC, 'f16_names.h')] if f16 else []
             cmd = [hipcc] + FLAGS + EXTRA_FLAGS.get(os.path.basename(src), []) + extra + ['-c', src, '-o', obj]
             if verbose:
@@ -70,7 +73,7 @@ def _build_locked(srcs, hdrs, force, verbose):
             if r.returncode != 0:
                 raise RuntimeError(f'hipcc failed on {src}:\n{r.stderr}')
             if verbose and r.stderr.strip():
-                print(r.stderr, file=sys.stderr)
+                print('\n'.join(ln for ln in r.stderr.splitlines() if 'packed-fp32-ops' not in ln), file=sys.stderr)
         return obj
 
     jobs = [(src, False) for src in srcs] + [(os.path.join(CSRC, f), True) for f in F16_SOURCES]

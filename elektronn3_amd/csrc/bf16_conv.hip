@@ -215,7 +215,7 @@ __global__ __launch_bounds__(256, (CH == 16 || BD <= 2) ? 3 : 2) void conv_b16_k
     // Everything outside the MFMA phase costs a wave ~13-24 cycles per vector instruction while the CU's other workgroups run their MFMAs
     // (profiles/r03_bf16_conv_experiments.md), so the epilogue is written for few instructions: the two run-time choices -- folded scale / shift
     // + ReLU or bias, interior brick or a brick that sticks out of the volume -- select one of four straight-line bodies (no per-element
-    // branches or selects), four channels at a time as vectors (packed fp32 ops, packed conversions).
+    // branches or selects), four channels at a time as vectors (packed conversions).
     float ssum[CO_T][16], ssq[CO_T][16];
     const bool want_stats = a.stats != nullptr;
     const bool interior = d0 + G::DZ <= a.D && h0 + G::BH <= a.H && w0 + G::BW <= a.W;

@@ -69,8 +69,7 @@ __global__ __launch_bounds__(256) void conv_small_fwd_kernel(const ConvSmallArgs
             for (int u = 0; u < 4; ++u) { const int idx = i0 + u * 256 + tid; if (idx < a.Cin * T * 32) ws[idx] = wv4[u]; }
         }
         __syncthreads();
-        // the 8 x 4 accumulators as pairs: hipcc packs the <2 x float> fma into v_pk_fma_f32 (two FMAs per lane and issue slot: the scalar form of
-        // this loop was FMA-issue bound, 1.8 G v_fma_f32 at 4 cycles per wave); a (kd, kh) row of the run = 10 halo values = three ds_read_b128
+        // the 8 x 4 accumulators as pairs (the library is built without packed fp32 instructions: each pair is two v_fma_f32); a (kd, kh) row of the run = 10 halo values = three ds_read_b128
         // instead of 24 ds_read_b32
         f32x2 alo[8], ahi[8];
 #pragma unroll

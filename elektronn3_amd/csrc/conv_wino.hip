@@ -115,7 +115,7 @@ __global__ __launch_bounds__(256, 1) void conv3_wino_kernel(const ConvArgs a) {
 
     // ---- read plan of lane (tile i = j, half hf): tile (td, th, tw) = (j >> 4, (j >> 3) & 1, j & 7), plane (td, pd = wave)
     float m1 = -1.f;
-    asm volatile("" : "+s"(m1));     // opaque -1: a + m1*b becomes v_pk_fma_f32 (hipcc only packs fadd/ffma, never fsub)
+    asm volatile("" : "+s"(m1));     // opaque -1: a - b as one fma, the same instruction as its neighbours
     const int ttd = j >> 4, tth = (j >> 3) & 1, ttw = j & 7;
     const int lbase = (ttd * 4 + wave) * W_PLANE + (tth * 9 + ttw) * 8;
     // rows h = 0,1 of the tile have zh/2 = th, rows 2,3 have th + 1: the swizzle bit differs between the two

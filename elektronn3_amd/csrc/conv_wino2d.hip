@@ -82,7 +82,7 @@ __global__ __launch_bounds__(256, 2) void conv2_wino_kernel(const ConvArgs a) {
     const int hb = wave == 0 ? 2 : (wave == 1 ? 2 : (wave == 2 ? 1 : 3));
     const float sgn = wave == 1 ? 1.f : -1.f;
     float m1 = -1.f;
-    asm volatile("" : "+s"(m1));     // opaque -1: a + m1*b becomes v_pk_fma_f32 (hipcc only packs fadd/ffma, never fsub)
+    asm volatile("" : "+s"(m1));     // opaque -1: a - b as one fma, the same instruction as its neighbours
     const int tth = j >> 3, ttw = j & 7;
     auto row_base = [&](int h) {     // LDS float offset of window row h, column 0 (w adds an immediate), this lane's 16-B half
         const int b = tth + (h >> 1);

@@ -160,7 +160,7 @@ __device__ __forceinline__ void wgrad_wino_segment(const WSeg& a, float* const s
     //   block 3:    starts with the brick's barrier (DMA of b + 1 landed, every wave done reading stage b); its MFMAs cover the scalar
     //               set-up of brick b + 2 and the LDS reads of block 0 of brick b + 1 -- no read is exposed after the barrier.
     static_assert(G_NV * 128 < 65536 && 2 * G_MV * 128 < 65536, "LDS read offsets must fit the 16-bit immediate");
-    // The transforms run PACKED (v_pk_add / v_pk_fma_f32: two lanes of work per VALU slot, ~7.9 vs 2 x 6.1 cycles).  The pairing that needs
+    // The transforms run on PAIRS (two scalar instructions each: the library is built without packed fp32).  The pairing that needs
     // no register moves and no duplicate loads: a block handles the lane's tiles (hc = 0, tl) and (hc = 1, tl) of a tile row -- w windows
     // 4 hc + 2 tl + [0, 4), disjoint -- as elements 0 / 1 of every pair; every pass is element-wise in the pair and the MFMA operands of
     // k-step s = 2 hc + tl are the halves of the result pairs.
