@@ -136,6 +136,12 @@ _SIG = {
     'e3_bn_bwd_workspace_bytes': (c_size_t, [_I, _I, _I, _I, _I]),
     'e3_bn_relu_bwd': (_I, [_P, _P, _I, _P, _P, _P, _P, _P, _P, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I,
                             _P, _I, _P, _P, _P, _P, c_size_t]),
+    'e3_group_norm_workspace_bytes': (c_size_t, [_I, _I, _I, _I, _I, _I]),
+    'e3_group_norm_act_fwd': (_I, [_P, _I, _P, _I, _P, _P, _F, _F, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P, c_size_t]),
+    'e3_group_norm_act_apply': (_I, [_P, _I, _P, _I, _P, _P, _P, _P, _P, _P, _F, _P, _I, _I, _I, _I, _I, _I, _I]),
+    'e3_group_norm_act_bwd': (_I, [_P, _I, _P, _I, _P, _P, _P, _P, _P, _P, _F, _P, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P, c_size_t]),
+    'e3_checkpoint8_pack': (_I, [_P, _I, _P, _I, c_int64, _I, _P, _P]),
+    'e3_checkpoint8_unpack': (_I, [_P, _I, _P, _P, c_int64, _I, _P, _I]),
     'e3_conv1_fwd': (_I, [_P, _P, _I, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I]),
     'e3_conv1_bwd_workspace_bytes': (c_size_t, [_I, _I, _I, _I, _I, _I]),
     'e3_conv1_bwd': (_I, [_P, _P, _I, _I, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _P, c_size_t]),

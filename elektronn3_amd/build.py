@@ -14,11 +14,11 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, 'csrc')
 OUT = os.path.join(HERE, 'libe3unet.so')
 OBJDIR = os.path.join(HERE, 'build')
-SOURCES = ['conv_mfma.hip', 'conv_v3.hip', 'conv_wino.hip', 'conv_wino4.hip', 'conv_wino2d.hip', 'upconv_gemm.hip', 'wgrad_mfma.hip', 'wgrad_wino.hip', 'wgrad_wino2d.hip', 'conv_small.hip', 'elementwise.hip', 'loss.hip', 'optim.hip', 'api.cpp', 'unet_plan.cpp',
+SOURCES = ['conv_mfma.hip', 'conv_v3.hip', 'conv_wino.hip', 'conv_wino4.hip', 'conv_wino2d.hip', 'upconv_gemm.hip', 'wgrad_mfma.hip', 'wgrad_wino.hip', 'wgrad_wino2d.hip', 'conv_small.hip', 'elementwise.hip', 'loss.hip', 'optim.hip', 'checkpoint8.hip', 'group_norm.hip', 'api.cpp', 'unet_plan.cpp',
            'attention.hip', 'bf16_conv.hip', 'bf16_wgrad.hip', 'bf16_upconv.hip', 'bf16_ew.hip', 'bf16_first.hip', 'api_bf16.cpp', 'unet_bf16.cpp']
 # the 16-bit path is compiled a second time for IEEE half (-DE3_F16, external symbols renamed by f16_names.h; see csrc/bf16.h)
 F16_SOURCES = ['bf16_conv.hip', 'bf16_wgrad.hip', 'bf16_upconv.hip', 'bf16_ew.hip', 'bf16_first.hip', 'api_bf16.cpp', 'unet_bf16.cpp']
-HEADERS = ['common.h', 'kernels.h', 'brick_order.h', 'bf16.h', 'f16_names.h', 'plan_internal.h', os.path.join('..', '..', 'include', 'e3unet.h')]
+HEADERS = ['common.h', 'kernels.h', 'brick_order.h', 'bf16.h', 'f16_names.h', 'plan_internal.h', 'checkpoint8.h', os.path.join('..', '..', 'include', 'e3unet.h')]
 # No packed fp32 instructions (v_pk_add / mul / fma_f32), which hipcc -O3 forms from ordinary float code: some of their forms give wrong results on MI355X
 # now and then, without an error.  (The host pass warns that it does not know the feature.)  What they were worth, same box: fp32 training step 11.02 -> 11.65 ms,
 # Predictor tile 6.36 -> 6.87 ms; 16-bit step unchanged.

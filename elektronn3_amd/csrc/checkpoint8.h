@@ -1,0 +1,130 @@
+// Element access of the normalisation kernels (group_norm.hip) and the 8-bit activation checkpoints (checkpoint8.hip).
+//
+// An 8-bit checkpoint of a channels-last tensor cuts its packed [N][D][H][W][C] elements into blocks of 64.  A block keeps
+//     q = round_to_even(x * (127 / amax))  in int8,   scale = amax * (1 / 127)  in fp32,   and stands for  fp32(q * scale),
+// with amax the block's largest magnitude and every operation rounded to fp32 (so that two implementations agree bit for bit).  Symmetric, because zero has to
+// stay zero (a ReLU's border); 64 elements, because a block is then 8 lanes of 8 elements (16-byte pieces of a 16-bit tensor) and the scales cost 1/16 of the
+// codes.  The step is amax / 127, the error of an element at most half of it.  amax < 2^-110: the block is kept as zeros (scale 0; 127 / amax would
+// overflow).  A block that holds a NaN or an infinity gets scale NaN: all of it comes back as NaN, so that a diverged activation stays visible.
+#pragma once
+#include "common.h"
+
+namespace e3n {
+
+constexpr int DT_F32 = 0, DT_BF16 = 1, DT_F16 = 2;         // E3_DT_* of include/e3unet.h
+constexpr int CK_BLOCK = 64;
+constexpr float CK_TINY = 0x1p-110f;
+
+typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
+
+template <int DT> struct Elem { typedef unsigned short T; };
+template <> struct Elem<DT_F32> { typedef float T; };
+
+template <int DT> __device__ __forceinline__ float to_f32(typename Elem<DT>::T v) {
+    if constexpr (DT == DT_F32) return v;
+    else if constexpr (DT == DT_BF16) return __uint_as_float((unsigned)v << 16);
+    else return (float)__builtin_bit_cast(_Float16, v);
+}
+template <int DT> __device__ __forceinline__ typename Elem<DT>::T from_f32(float f) {       // round to nearest even; NaN stays NaN
+    if constexpr (DT == DT_F32) return f;
+    else if constexpr (DT == DT_BF16) return __builtin_bit_cast(unsigned short, (__bf16)f);
+    else return __builtin_bit_cast(unsigned short, (_Float16)f);
+}
+
+// V consecutive channels of a voxel as they lie in memory: V = 8 with 16-byte accesses (C, row length and address in multiples of 8 elements / 16 bytes), or V = 1
+template <int DT, int V> struct Raw { typename Elem<DT>::T v; };
+template <> struct Raw<DT_F32, 8> { f32x4 lo, hi; };
+template <> struct Raw<DT_BF16, 8> { u16x8 v; };
+template <> struct Raw<DT_F16, 8> { u16x8 v; };
+
+template <int DT, int V> __device__ __forceinline__ Raw<DT, V> load_raw(const typename Elem<DT>::T* p) {
+    Raw<DT, V> r;
+    if constexpr (V == 1) r.v = *p;
+    else if constexpr (DT == DT_F32) { r.lo = *reinterpret_cast<const f32x4*>(p); r.hi = *reinterpret_cast<const f32x4*>(p + 4); }
+    else r.v = *reinterpret_cast<const u16x8*>(p);
+    return r;
+}
+template <int DT, int V> __device__ __forceinline__ void unpack_raw(const Raw<DT, V>& r, float (&f)[V]) {
+    if constexpr (V == 1) f[0] = to_f32<DT>(r.v);
+    else if constexpr (DT == DT_F32) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { f[e] = r.lo[e]; f[e + 4] = r.hi[e]; }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = to_f32<DT>(r.v[e]);
+    }
+}
+template <int DT, int V> __device__ __forceinline__ void store_f32(typename Elem<DT>::T* p, const float (&f)[V]) {
+    if constexpr (V == 1) *p = from_f32<DT>(f[0]);
+    else if constexpr (DT == DT_F32) {
+        *reinterpret_cast<f32x4*>(p) = f32x4{f[0], f[1], f[2], f[3]};
+        *reinterpret_cast<f32x4*>(p + 4) = f32x4{f[4], f[5], f[6], f[7]};
+    } else {
+        u16x8 o;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = from_f32<DT>(f[e]);
+        *reinterpret_cast<u16x8*>(p) = o;
+    }
+}
+
+// V codes of a checkpoint and their scale
+template <int V> struct RawQ { uint2 q; float s; };
+template <> struct RawQ<1> { signed char q; float s; };
+template <int V> __device__ __forceinline__ RawQ<V> load_q(const signed char* q, const float* scale, size_t e) {       // e: flat element, a multiple of V
+    RawQ<V> r;
+    if constexpr (V == 1) r.q = q[e]; else r.q = *reinterpret_cast<const uint2*>(q + e);
+    r.s = scale[e / CK_BLOCK];
+    return r;
+}
+template <int V> __device__ __forceinline__ void unpack_q(const RawQ<V>& r, float (&f)[V]) {
+#pragma clang fp contract(off)          // (the value is the ROUNDED product wherever it is used: fused into a reader's x - mean it would be another one)
+    if constexpr (V == 1) f[0] = (float)r.q * r.s;
+    else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            f[e] = (float)(signed char)(r.q.x >> (8 * e)) * r.s;
+            f[e + 4] = (float)(signed char)(r.q.y >> (8 * e)) * r.s;
+        }
+    }
+}
+
+// A block's scale and codes from the values of its lanes: 64 / V consecutive lanes of a wave hold one block, V consecutive elements each (lanes outside the tensor
+// pass zeros).  Magnitudes are compared as integers, where infinities and NaNs are the largest.  EVERY lane of the wave has to get here.
+template <int V> struct Codes { signed char q[V]; float scale; };
+template <int V> __device__ __forceinline__ Codes<V> encode_block(const float (&f)[V]) {
+    unsigned m = 0;
+#pragma unroll
+    for (int e = 0; e < V; ++e) m = max(m, __float_as_uint(f[e]) & 0x7fffffffu);
+#pragma unroll
+    for (int o = 1; o < CK_BLOCK / V; o <<= 1) m = max(m, (unsigned)__shfl_xor((int)m, o));
+    const float amax = __uint_as_float(m);
+    const bool none = m < __float_as_uint(CK_TINY), bad = m >= 0x7f800000u;
+    const float inv = (none || bad) ? 0.f : 127.f / amax;
+    Codes<V> c;
+    c.scale = none ? 0.f : (bad ? __uint_as_float(0x7fc00000u) : amax * (1.f / 127.f));
+#pragma unroll
+    for (int e = 0; e < V; ++e) c.q[e] = (none || bad) ? (signed char)0 : (signed char)(int)rintf(f[e] * inv);
+    return c;
+}
+template <int V> __device__ __forceinline__ void store_codes(const Codes<V>& c, signed char* q, float* scale, size_t e) {
+    if constexpr (V == 1) q[e] = c.q[0];
+    else {
+        unsigned lo = 0, hi = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) { lo |= (unsigned)(unsigned char)c.q[k] << (8 * k); hi |= (unsigned)(unsigned char)c.q[k + 4] << (8 * k); }
+        *reinterpret_cast<uint2*>(q + e) = make_uint2(lo, hi);
+    }
+    if (e % CK_BLOCK == 0) scale[e / CK_BLOCK] = c.scale;
+}
+
+inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+// whether the rows of a view allow 16-byte pieces of 8 channels
+inline bool rows_by_8(int dt, const void* p, int ldc, int C) {
+    return C % 8 == 0 && aligned16(p) && ldc % (dt == DT_F32 ? 4 : 8) == 0;
+}
+
+}  // namespace e3n
+
+// (stream, type, view of x, its checkpoint): launchers shared with the fused forms
+int launch_checkpoint8_pack(int dt, const void* x, int x_ldc, long long vox, int C, signed char* q, float* scale, hipStream_t s);
+int launch_checkpoint8_unpack(int dt, const signed char* q, const float* scale, long long vox, int C, void* y, int y_ldc, hipStream_t s);

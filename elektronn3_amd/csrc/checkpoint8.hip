@@ -1,0 +1,139 @@
+// 8-bit activation checkpoints: a tensor into codes and block scales, and back (the format: checkpoint8.h).
+//
+// Both are one streaming pass: 4 + 1.06 bytes per fp32 element, 2 + 1.06 per 16-bit element, a few operations each: HBM-bound.
+#include "checkpoint8.h"
+
+#include "../../include/e3unet.h"
+
+using namespace e3n;
+
+namespace {
+
+constexpr int BT = 256;
+
+// flat piece -> (voxel row, first channel).  DENSE: the rows follow each other without a gap, the view is one flat array.
+template <int V, bool DENSE> __device__ __forceinline__ size_t piece_offset(size_t e, int C, int ldc) {
+    if constexpr (DENSE) return e;
+    else {
+        const size_t v = e < 0xffffffffu ? (size_t)((unsigned)e / (unsigned)C) : e / (size_t)C;
+        return v * (size_t)ldc + (e - v * (size_t)C);
+    }
+}
+
+template <int DT, int V, bool DENSE>
+__global__ __launch_bounds__(BT) void checkpoint8_pack_kernel(const typename Elem<DT>::T* __restrict__ x, int ldc, int C, size_t n,
+                                                              signed char* __restrict__ q, float* __restrict__ scale) {
+    constexpr int U = 4;                                     // pieces in flight per lane
+    const size_t step = (size_t)gridDim.x * BT * V;
+    // (the loop's condition is the workgroup's: every lane of a wave reaches the reduction inside encode_block)
+    for (size_t b0 = (size_t)blockIdx.x * BT * V; b0 < n; b0 += U * step) {
+        Raw<DT, V> raw[U]; bool ok[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const size_t e = b0 + u * step + (size_t)threadIdx.x * V;
+            ok[u] = e < n;
+            raw[u] = Raw<DT, V>{};
+            if (ok[u]) raw[u] = load_raw<DT, V>(x + piece_offset<V, DENSE>(e, C, ldc));
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            float f[V];
+            unpack_raw<DT, V>(raw[u], f);
+            const Codes<V> c = encode_block<V>(f);
+            if (ok[u]) store_codes<V>(c, q, scale, b0 + u * step + (size_t)threadIdx.x * V);
+        }
+    }
+}
+
+template <int DT, int V, bool DENSE>
+__global__ __launch_bounds__(BT) void checkpoint8_unpack_kernel(const signed char* __restrict__ q, const float* __restrict__ scale, size_t n, int C, int ldc,
+                                                                typename Elem<DT>::T* __restrict__ y) {
+    constexpr int U = 4;
+    const size_t step = (size_t)gridDim.x * BT * V;
+    for (size_t e0 = ((size_t)blockIdx.x * BT + threadIdx.x) * V; e0 < n; e0 += U * step) {
+        RawQ<V> raw[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) { raw[u] = RawQ<V>{}; if (e0 + u * step < n) raw[u] = load_q<V>(q, scale, e0 + u * step); }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            float f[V];
+            unpack_q<V>(raw[u], f);
+            if (e0 + u * step < n) store_f32<DT, V>(y + piece_offset<V, DENSE>(e0 + u * step, C, ldc), f);
+        }
+    }
+}
+
+unsigned grid_for(size_t n, int V) {
+    const size_t blocks = (n + (size_t)BT * V - 1) / ((size_t)BT * V);
+    return (unsigned)(blocks < 2048 ? blocks : 2048);       // 8 workgroups of 4 waves per CU, grid-stride beyond
+}
+
+template <int DT, int V>
+void pack_typed(const void* x, int ldc, size_t n, int C, signed char* q, float* scale, hipStream_t s) {
+    typedef const typename Elem<DT>::T* P;
+    if (ldc == C) hipLaunchKernelGGL((checkpoint8_pack_kernel<DT, V, true>), dim3(grid_for(n, V)), dim3(BT), 0, s, (P)x, ldc, C, n, q, scale);
+    else hipLaunchKernelGGL((checkpoint8_pack_kernel<DT, V, false>), dim3(grid_for(n, V)), dim3(BT), 0, s, (P)x, ldc, C, n, q, scale);
+}
+template <int DT, int V>
+void unpack_typed(const signed char* q, const float* scale, size_t n, int C, void* y, int ldc, hipStream_t s) {
+    typedef typename Elem<DT>::T* P;
+    if (ldc == C) hipLaunchKernelGGL((checkpoint8_unpack_kernel<DT, V, true>), dim3(grid_for(n, V)), dim3(BT), 0, s, q, scale, n, C, ldc, (P)y);
+    else hipLaunchKernelGGL((checkpoint8_unpack_kernel<DT, V, false>), dim3(grid_for(n, V)), dim3(BT), 0, s, q, scale, n, C, ldc, (P)y);
+}
+
+// a flat tensor of rows without gaps is cut at multiples of 8 whatever its channel count
+bool by_8(int dt, const void* p, int ldc, int C, size_t n, const void* q) {
+    return ((uintptr_t)q & 7) == 0 && (ldc == C ? n % 8 == 0 && aligned16(p) : rows_by_8(dt, p, ldc, C));
+}
+
+}  // namespace
+
+int launch_checkpoint8_pack(int dt, const void* x, int x_ldc, long long vox, int C, signed char* q, float* scale, hipStream_t s) {
+    const size_t n = (size_t)vox * C;
+    if (n == 0) return E3_OK;
+    const bool v8 = by_8(dt, x, x_ldc, C, n, q);
+    switch (dt * 2 + v8) {
+        case 0: pack_typed<DT_F32, 1>(x, x_ldc, n, C, q, scale, s); break;
+        case 1: pack_typed<DT_F32, 8>(x, x_ldc, n, C, q, scale, s); break;
+        case 2: pack_typed<DT_BF16, 1>(x, x_ldc, n, C, q, scale, s); break;
+        case 3: pack_typed<DT_BF16, 8>(x, x_ldc, n, C, q, scale, s); break;
+        case 4: pack_typed<DT_F16, 1>(x, x_ldc, n, C, q, scale, s); break;
+        default: pack_typed<DT_F16, 8>(x, x_ldc, n, C, q, scale, s); break;
+    }
+    E3_CHECK_HIP(hipGetLastError());
+    return E3_OK;
+}
+
+int launch_checkpoint8_unpack(int dt, const signed char* q, const float* scale, long long vox, int C, void* y, int y_ldc, hipStream_t s) {
+    const size_t n = (size_t)vox * C;
+    if (n == 0) return E3_OK;
+    const bool v8 = by_8(dt, y, y_ldc, C, n, q);
+    switch (dt * 2 + v8) {
+        case 0: unpack_typed<DT_F32, 1>(q, scale, n, C, y, y_ldc, s); break;
+        case 1: unpack_typed<DT_F32, 8>(q, scale, n, C, y, y_ldc, s); break;
+        case 2: unpack_typed<DT_BF16, 1>(q, scale, n, C, y, y_ldc, s); break;
+        case 3: unpack_typed<DT_BF16, 8>(q, scale, n, C, y, y_ldc, s); break;
+        case 4: unpack_typed<DT_F16, 1>(q, scale, n, C, y, y_ldc, s); break;
+        default: unpack_typed<DT_F16, 8>(q, scale, n, C, y, y_ldc, s); break;
+    }
+    E3_CHECK_HIP(hipGetLastError());
+    return E3_OK;
+}
+
+extern "C" {
+
+int e3_checkpoint8_pack(void* stream, int dtype, const void* x, int x_ldc, long long voxels, int C, signed char* q, float* scale) {
+    E3_REQUIRE(dtype >= 0 && dtype <= 2, E3_ERR_INVALID, "dtype must be E3_DT_F32, E3_DT_BF16 or E3_DT_F16");
+    E3_REQUIRE(C >= 1 && voxels >= 0 && x_ldc >= C, E3_ERR_INVALID, "bad sizes");
+    E3_REQUIRE(voxels == 0 || (x && q && scale), E3_ERR_INVALID, "null argument");
+    return launch_checkpoint8_pack(dtype, x, x_ldc, voxels, C, q, scale, (hipStream_t)stream);
+}
+
+int e3_checkpoint8_unpack(void* stream, int dtype, const signed char* q, const float* scale, long long voxels, int C, void* y, int y_ldc) {
+    E3_REQUIRE(dtype >= 0 && dtype <= 2, E3_ERR_INVALID, "dtype must be E3_DT_F32, E3_DT_BF16 or E3_DT_F16");
+    E3_REQUIRE(C >= 1 && voxels >= 0 && y_ldc >= C, E3_ERR_INVALID, "bad sizes");
+    E3_REQUIRE(voxels == 0 || (y && q && scale), E3_ERR_INVALID, "null argument");
+    return launch_checkpoint8_unpack(dtype, q, scale, voxels, C, y, y_ldc, (hipStream_t)stream);
+}
+
+}  // extern "C"

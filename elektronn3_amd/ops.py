@@ -327,3 +327,207 @@ def convT_wgrad_bf16(x, dy):
     check(L.e3_convT_wgrad_bf16(stream_ptr(x.device), ptr(x), _ldc(x), Cin, ptr(dy), _ldc(dy), Cout, ptr(dw), N, D, H, W, Do, Ho, Wo,
                                 ptr(ws), c_size_t(ws.numel())))
     return dw
+
+
+# ------------------------------------------------------------------ group norm with an activation, 8-bit activation checkpoints
+_DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}       # E3_DT_*
+
+
+def _chk_any(t, name, like=None):
+    """An fp32 / bf16 / fp16 NDHWC view on a ROCm device (with the shape, type and device of `like`)."""
+    if not isinstance(t, torch.Tensor) or t.dtype not in _DT:
+        raise ValueError(f'{name}: expected a float32, bfloat16 or float16 tensor')
+    if not t.is_cuda:
+        raise ValueError(f'{name}: expected a CUDA tensor (the HIP path has no CPU fallback)')
+    if t.dim() != 5:
+        raise ValueError(f'{name}: expected a 5D (N, D, H, W, C) tensor, got {t.dim()}D')
+    if like is not None and (tuple(t.shape) != tuple(like.shape) or t.dtype != like.dtype or t.device != like.device):
+        raise ValueError(f'{name}: expected shape {tuple(like.shape)}, {like.dtype} on {like.device}, got {tuple(t.shape)}, {t.dtype} on {t.device}')
+    return _ldc(t) if t.numel() else max(t.shape[4], 1)
+
+
+def _chk_out(out, ins, name='out'):
+    """`out` may be one of the inputs itself (the same view); a view that overlaps one otherwise would be read after it was written."""
+    lo = out.data_ptr()
+    hi = lo + ((out.shape[0] - 1) * out.stride(0) + (out.shape[1] - 1) * out.stride(1) + (out.shape[2] - 1) * out.stride(2)
+               + (out.shape[3] - 1) * out.stride(3) + out.shape[4]) * out.element_size() if out.numel() else lo
+    for t in ins:
+        if t is None or t.numel() == 0 or (t.data_ptr() == lo and t.dtype == out.dtype and t.stride() == out.stride()):
+            continue
+        a = t.data_ptr()
+        b = a + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+        # (the two halves of a concat buffer interleave in memory without sharing an element: rows of the same buffer, other channels)
+        if a < hi and lo < b and not _disjoint_channels(t, out):
+            raise ValueError(f'{name} overlaps an input without being the same view')
+
+
+def _disjoint_channels(t, out):
+    if t.dtype != out.dtype or t.dim() != 5:
+        return False
+    ldc, d = _ldc(out), (t.data_ptr() - out.data_ptr())
+    if _ldc(t) != ldc or d % t.element_size():
+        return False
+    d = (d // t.element_size()) % ldc
+    return d >= out.shape[4] and d + t.shape[4] <= ldc
+
+
+def _chk_vec(t, n, name, device):
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.numel() != n or t.device != device:
+        raise ValueError(f'{name}: expected {n} float32 values on {device}')
+    return t.contiguous()
+
+
+def _act_slope(activation):
+    """Slope code of the C ABI from an activation's name or module (those of UNet(activation=...)); nn.PReLU and nn.RReLU are not covered."""
+    from .unet import _activation_slope
+    slope = _activation_slope(activation)
+    if slope is None or slope == 3.0 or activation == 'rrelu' or isinstance(activation, torch.nn.RReLU):
+        raise NotImplementedError(f"activation {activation!r}: 'relu', 'leaky', 'lin', 'silu' or their modules")
+    return slope
+
+
+class Checkpoint8:
+    """An (N, D, H, W, C) activation kept in 8 bits: ``q`` (int8, one code per element in packed NDHWC order) and ``scale`` (float32, one per 64
+    elements).  It stands for ``q * scale`` (3.76 times smaller than float32, 1.88 times than a 16-bit type); an element is off by at most half
+    a step, ``amax / 254`` of its block's largest magnitude.  A block with a NaN or an infinity stands for NaNs.  Made by :func:`checkpoint8` or
+    :func:`group_norm_act`; read by :func:`checkpoint8_restore`, :func:`group_norm_act_apply` and :func:`group_norm_act_bwd`."""
+    __slots__ = ('q', 'scale', 'shape', 'dtype')
+
+    def __init__(self, q, scale, shape, dtype):
+        shape = torch.Size(int(s) for s in shape)
+        n = shape.numel()
+        if len(shape) != 5 or dtype not in _DT:
+            raise ValueError('Checkpoint8: expected the (N, D, H, W, C) shape and the float32, bfloat16 or float16 type of the tensor it stands for')
+        if q.dtype != torch.int8 or q.numel() != n or not q.is_contiguous():
+            raise ValueError(f'Checkpoint8: q: expected {n} contiguous int8 codes')
+        if scale.dtype != torch.float32 or scale.numel() != -(-n // 64) or not scale.is_contiguous() or scale.device != q.device:
+            raise ValueError(f'Checkpoint8: scale: expected {-(-n // 64)} contiguous float32 values on {q.device}')
+        if not q.is_cuda:
+            raise ValueError('Checkpoint8: expected CUDA tensors (the HIP path has no CPU fallback)')
+        self.q, self.scale, self.shape, self.dtype = q, scale, shape, dtype
+
+    @property
+    def device(self):
+        return self.q.device
+
+    @property
+    def nbytes(self):
+        return self.q.numel() + 4 * self.scale.numel()
+
+    def numel(self):
+        return self.q.numel()
+
+    def __repr__(self):
+        return f'Checkpoint8(shape={tuple(self.shape)}, dtype={self.dtype}, device={self.device})'
+
+
+def _new_checkpoint(x):
+    n = x.numel()
+    return Checkpoint8(torch.empty(n, dtype=torch.int8, device=x.device), torch.empty(-(-n // 64), dtype=torch.float32, device=x.device), x.shape, x.dtype)
+
+
+def checkpoint8(x):
+    """Keeps an activation (float32 / bfloat16 / float16 NDHWC view) in 8 bits; see :class:`Checkpoint8`."""
+    ldc = _chk_any(x, 'x')
+    ck = _new_checkpoint(x)
+    with torch.cuda.device(x.device):
+        check(_lib.load().e3_checkpoint8_pack(stream_ptr(x.device), _DT[x.dtype], ptr(x), ldc, x.numel() // max(x.shape[4], 1), x.shape[4] or 1, ptr(ck.q), ptr(ck.scale)))
+    return ck
+
+
+def checkpoint8_restore(ck, out=None):
+    """The tensor that a :class:`Checkpoint8` stands for, rounded to its type (into ``out``, an NDHWC view, if given)."""
+    if not isinstance(ck, Checkpoint8):
+        raise ValueError('expected a Checkpoint8')
+    y = out if out is not None else torch.empty(ck.shape, dtype=ck.dtype, device=ck.device)
+    ldc = _chk_any(y, 'out', like=ck)
+    with torch.cuda.device(ck.device):
+        check(_lib.load().e3_checkpoint8_unpack(stream_ptr(ck.device), _DT[ck.dtype], ptr(ck.q), ptr(ck.scale), ck.numel() // max(ck.shape[4], 1), ck.shape[4] or 1,
+                                                ptr(y), ldc))
+    return y
+
+
+def _source(x):
+    """(x pointer, ldc, q pointer, scale pointer) of a tensor or a checkpoint of it."""
+    if isinstance(x, Checkpoint8):
+        return None, 0, ptr(x.q), ptr(x.scale)
+    return ptr(x), _chk_any(x, 'x'), None, None
+
+
+def _gn_dims(x, num_groups):
+    N, D, H, W, C = x.shape
+    if min(x.shape) < 1:
+        raise ValueError(f'x: expected at least one element, got shape {tuple(x.shape)}')
+    if num_groups < 1 or C % num_groups != 0:
+        raise ValueError('num_channels must be divisible by num_groups')
+    return N, D, H, W, C, num_groups
+
+
+def _stats(x, mean, rstd):
+    if mean.dim() != 2 or mean.shape[0] != x.shape[0]:
+        raise ValueError(f'mean: expected shape ({x.shape[0]}, num_groups)')
+    n = mean.numel()
+    return _chk_vec(mean, n, 'mean', x.device), _chk_vec(rstd, n, 'rstd', x.device), mean.shape[1]
+
+
+def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, activation='relu', checkpoint=False, out=None):
+    """``act(group_norm(x, num_groups, weight, bias, eps))`` over a float32 / bfloat16 / float16 NDHWC view (weight, bias: float32 (C,)), with the statistics
+    that the backward needs: ``(y, mean, rstd)``, mean and rstd (N, num_groups) float32.  ``checkpoint=True`` also keeps ``x`` in 8 bits on the way:
+    ``(y, mean, rstd, Checkpoint8)``.  ``out`` may be ``x`` itself."""
+    slope = _act_slope(activation)
+    ldc = _chk_any(x, 'x')
+    dims = _gn_dims(x, num_groups)
+    weight, bias = _chk_vec(weight, x.shape[4], 'weight', x.device), _chk_vec(bias, x.shape[4], 'bias', x.device)
+    if not eps >= 0:
+        raise ValueError('eps must not be negative')
+    y = out if out is not None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y_ldc = _chk_any(y, 'out', like=x)
+    if out is not None:
+        _chk_out(out, (x,))
+    L = _lib.load()
+    mean, rstd = (torch.empty((x.shape[0], num_groups), dtype=torch.float32, device=x.device) for _ in range(2))
+    ck = _new_checkpoint(x) if checkpoint else None
+    ws = _ws(L.e3_group_norm_workspace_bytes(*dims), x.device)
+    with torch.cuda.device(x.device):
+        check(L.e3_group_norm_act_fwd(stream_ptr(x.device), _DT[x.dtype], ptr(x), ldc, ptr(weight), ptr(bias), float(eps), slope, ptr(y), y_ldc, ptr(mean), ptr(rstd),
+                                      ptr(ck.q) if ck else None, ptr(ck.scale) if ck else None, *dims, ptr(ws), c_size_t(ws.numel())))
+    return (y, mean, rstd, ck) if checkpoint else (y, mean, rstd)
+
+
+def group_norm_act_apply(x, mean, rstd, weight=None, bias=None, activation='relu', out=None):
+    """``y`` of :func:`group_norm_act` from its statistics and its input or the input's :class:`Checkpoint8` (the activation recomputed in a backward
+    pass; a checkpoint's values enter in float32)."""
+    slope = _act_slope(activation)
+    src = _source(x)
+    mean, rstd, G = _stats(x, mean, rstd)
+    dims = _gn_dims(x, G)
+    weight, bias = _chk_vec(weight, x.shape[4], 'weight', x.device), _chk_vec(bias, x.shape[4], 'bias', x.device)
+    y = out if out is not None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y_ldc = _chk_any(y, 'out', like=x)
+    if out is not None and not isinstance(x, Checkpoint8):
+        _chk_out(out, (x,))
+    with torch.cuda.device(x.device):
+        check(_lib.load().e3_group_norm_act_apply(stream_ptr(x.device), _DT[x.dtype], *src, ptr(mean), ptr(rstd), ptr(weight), ptr(bias), slope, ptr(y), y_ldc, *dims))
+    return y
+
+
+def group_norm_act_bwd(x, mean, rstd, dy, weight=None, bias=None, activation='relu'):
+    """Gradients ``(dx, dweight, dbias)`` of :func:`group_norm_act` from its statistics and its input or the input's :class:`Checkpoint8`; dweight and
+    dbias are float32 (C,) whether or not the norm has parameters."""
+    slope = _act_slope(activation)
+    src = _source(x)
+    mean, rstd, G = _stats(x, mean, rstd)
+    dims = _gn_dims(x, G)
+    C = x.shape[4]
+    weight, bias = _chk_vec(weight, C, 'weight', x.device), _chk_vec(bias, C, 'bias', x.device)
+    dy_ldc = _chk_any(dy, 'dy', like=x)
+    L = _lib.load()
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dw, db = (torch.empty(C, dtype=torch.float32, device=x.device) for _ in range(2))
+    ws = _ws(L.e3_group_norm_workspace_bytes(*dims), x.device)
+    with torch.cuda.device(x.device):
+        check(L.e3_group_norm_act_bwd(stream_ptr(x.device), _DT[x.dtype], *src, ptr(mean), ptr(rstd), ptr(weight), ptr(bias), slope, ptr(dy), dy_ldc, ptr(dx), C,
+                                      ptr(dw), ptr(db), *dims, ptr(ws), c_size_t(ws.numel())))
+    return dx, dw, db

@@ -36,6 +36,11 @@ extern "C" {
 #define E3_ERR_UNSUPPORTED 3
 #define E3_ERR_WORKSPACE 4
 
+/* element types of the entry points that take one (`dtype`): fp32, bfloat16, IEEE half */
+#define E3_DT_F32 0
+#define E3_DT_BF16 1
+#define E3_DT_F16 2
+
 /* Message of the last failing call on this thread ("" if none). */
 const char* e3_last_error(void);
 /* Library version string, e.g. "e3unet 0.1 gfx950". */
@@ -259,6 +264,36 @@ int e3_bn_relu_bwd(void* stream, const float* x, int x_ldc, const float* mean, c
                    const float* scale, const float* shift, const float* g1, int g1_ldc, const float* gpool,
                    const float* a, int a_ldc, const float* pooled, int kd, int N, int D, int H, int W, int C,
                    float* dx, int dx_ldc, float* dgamma, float* dbeta, float* dxsum, void* workspace, size_t workspace_bytes);
+
+/* Group norm with an activation over NDHWC views of any `dtype` (nn.GroupNorm of get_normalization('group<G>') followed by get_activation,
+ * unet.py:77-105,183-199): groups of C / G consecutive channels of one sample,
+ *     y = act((x - mean) * rstd * gamma + beta),   rstd = (var + eps)^-1/2.
+ *   gamma, beta: [C] fp32, or NULL (1 and 0).  act_slope: 0 = ReLU, (0, 1) = LeakyReLU, 1 = identity, 2 = SiLU.
+ *   mean, rstd:  [N][G] fp32 outputs (inputs of _apply and _bwd).
+ *   q, q_scale:  NULL, or the 8-bit checkpoint of x that the same call writes (see e3_checkpoint8_pack; N*D*H*W*C codes).
+ *   workspace:   e3_group_norm_workspace_bytes() bytes, for both directions.
+ * y may be x itself (the same view), dx may be dy.  Statistics and sums are fp32 values of fp64 sums in a fixed order. */
+size_t e3_group_norm_workspace_bytes(int N, int D, int H, int W, int C, int G);
+int e3_group_norm_act_fwd(void* stream, int dtype, const void* x, int x_ldc, const float* gamma, const float* beta, float eps, float act_slope,
+                          void* y, int y_ldc, float* mean, float* rstd, signed char* q, float* q_scale,
+                          int N, int D, int H, int W, int C, int G, void* workspace, size_t workspace_bytes);
+/* y of the above from given statistics, and from x or (x == NULL) from its checkpoint: the activation recomputed in a backward pass. */
+int e3_group_norm_act_apply(void* stream, int dtype, const void* x, int x_ldc, const signed char* q, const float* q_scale,
+                            const float* mean, const float* rstd, const float* gamma, const float* beta, float act_slope,
+                            void* y, int y_ldc, int N, int D, int H, int W, int C, int G);
+/* Gradients of e3_group_norm_act_fwd from x or (x == NULL) from its checkpoint, whose values are used in fp32.  dgamma, dbeta: [C], either may
+ * be NULL.  The derivative of ReLU / LeakyReLU at 0 is that of the negative side. */
+int e3_group_norm_act_bwd(void* stream, int dtype, const void* x, int x_ldc, const signed char* q, const float* q_scale,
+                          const float* mean, const float* rstd, const float* gamma, const float* beta, float act_slope,
+                          const void* dy, int dy_ldc, void* dx, int dx_ldc, float* dgamma, float* dbeta,
+                          int N, int D, int H, int W, int C, int G, void* workspace, size_t workspace_bytes);
+
+/* 8-bit activation checkpoints (what UNet.forward_gradcp trades recomputation for, unet.py:918-935, trades precision for here): the packed
+ * [voxel][C] elements in blocks of 64; a block keeps q = round_to_even(x * (127 / amax)) and scale = amax * (1 / 127), amax its largest
+ * magnitude, each operation rounded to fp32, and stands for fp32(q * scale).  A block with amax < 2^-110 is kept as zeros; one that holds a
+ * NaN or an infinity comes back as NaN.  q: [voxels * C], scale: [ceil(voxels * C / 64)]. */
+int e3_checkpoint8_pack(void* stream, int dtype, const void* x, int x_ldc, long long voxels, int C, signed char* q, float* scale);
+int e3_checkpoint8_unpack(void* stream, int dtype, const signed char* q, const float* scale, long long voxels, int C, void* y, int y_ldc);
 
 /* conv_final: nn.Conv3d(C, Cout, 1)   [unet.py:178-180, 881, 912].  y and dy are NCDHW (module boundary). */
 int e3_conv1_fwd(void* stream, const float* a, int a_ldc, int C, const float* w, const float* bias, float* y_ncdhw,
