@@ -8,9 +8,11 @@
 // All kernels are streaming passes with one mapping: a thread keeps V consecutive channels (V = 8: 16-byte accesses; V = 1 for rows that do not allow them) and
 // walks the voxels of its workgroup's chunk, so that the per-channel constants stay in registers; consecutive threads take consecutive pieces of a voxel, then
 // consecutive voxels.  A workgroup works on one chunk of one sample and, for more than 512 pieces per voxel, on one tile of its channels.
-//   forward:   statistics (read x) -> finalise -> apply (read x, write y [, write the checkpoint])
-//   backward:  reduce (read x, dy) -> finalise -> apply (read x, dy, write dx)
-// Sums leave a workgroup as fp64 records [sample][chunk][..], merged in a fixed order: results do not depend on timing.
+//   forward:   statistics (read x) -> apply (read x, write y [, write the checkpoint])
+//   backward:  reduce (read x, dy) -> apply (read x, dy, write dx)
+// Sums leave a workgroup as fp64 records [sample][chunk][..], merged in a fixed order: results do not depend on timing.  Every workgroup of the apply pass
+// merges its sample's records itself (a few tens of KB out of L2, about 1 us) instead of waiting for a third launch in between; where the records of a
+// sample are more than MERGE_MAX a finalising launch does it.
 #include "checkpoint8.h"
 
 #include "../../include/e3unet.h"
@@ -36,12 +38,18 @@ struct GnArgs {
     int chunks; long long chunk;             // chunks of a sample, voxels of a chunk
     int unit;                                // channels that the statistics pass adds up before it writes them (divides cg and V)
     double* part;                            // records (sum, sum of squares) [N][chunks][C / unit] | (sum dz, sum dz h) [N][chunks][C]
+    double* gpart;                           // backward: (sum gamma dz, sum gamma dz h) [N][chunks][G], or nullptr
+    // apply passes that merge the records themselves (rec != nullptr)
+    const double* rec; int rec_chunks, rec_units, rec_per;      // [N][rec_chunks][rec_units] pairs, rec_per units to a group
+    double inv_m; float eps;
+    float* mean_out; float* rstd_out;        // forward: the statistics, written by the first workgroup of a sample
+    const double* cpart; float* dgamma; float* dbeta; int sum_wgs;      // backward: the first sum_wgs workgroups sum the channel records [N * rec_chunks][C]
 };
 
 struct Where { int n, tile, r, p, c; long long v0, v1; bool on; };
-template <int V> __device__ __forceinline__ Where where(const GnArgs& a) {
+template <int V> __device__ __forceinline__ Where where(const GnArgs& a, unsigned b) {
     Where w;
-    const unsigned b = blockIdx.x, t = b / a.tiles;
+    const unsigned t = b / a.tiles;
     w.tile = b % a.tiles;
     w.n = t / a.chunks;
     const int k = t % a.chunks;
@@ -81,12 +89,40 @@ template <typename T, typename F> __device__ __forceinline__ void sum_rows(const
     }
 }
 
+// Merges a sample's records [chunks][units] of pairs into sh[2 g], sh[2 g + 1] for its groups (per units each).  Threads read the records in memory order and
+// keep their unit; rows, then units of a group, are added in a fixed order.  sh: 2 blockDim + 2 units doubles at least.
+__device__ __forceinline__ void merge_records(const double* rec, int chunks, int units, int per, double* sh) {
+    const int rows = blockDim.x / units, T = rows * units, n = chunks * units;
+    double s = 0.0, t = 0.0;
+    if ((int)threadIdx.x < T)
+        for (int j = threadIdx.x; j < n; j += 4 * T) {
+            double2 v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) { v[k] = make_double2(0.0, 0.0); if (j + k * T < n) v[k] = *reinterpret_cast<const double2*>(rec + 2 * (size_t)(j + k * T)); }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) { s += v[k].x; t += v[k].y; }
+        }
+    double* sums = sh + 2 * blockDim.x;
+    if ((int)threadIdx.x < T) { sh[threadIdx.x] = s; sh[T + threadIdx.x] = t; }
+    __syncthreads();
+    sum_rows(sh, sh + T, rows, units, [&](int u, double x, double y) { sums[2 * u] = x; sums[2 * u + 1] = y; });
+    __syncthreads();
+    for (int g = threadIdx.x; g < units / per; g += blockDim.x) {
+        double x = 0.0, y = 0.0;
+        for (int k = 0; k < per; ++k) { x += sums[2 * (g * per + k)]; y += sums[2 * (g * per + k) + 1]; }
+        sh[2 * g] = x; sh[2 * g + 1] = y;
+    }
+    __syncthreads();
+}
+constexpr int MERGE_MAX = 4096;              // records of a sample that the apply pass merges itself (64 KB)
+constexpr int MERGE_UNITS = 128;             // ... of at most so many units (a workgroup has 192 threads or more)
+
 // ------------------------------------------------------------------------------------------------ forward
 // Sums and sums of squares in fp64: the variance is then a difference that loses nothing an fp32 input holds, whatever its mean.
 template <int DT, int V>
 __global__ __launch_bounds__(MAX_T) void gn_stats_kernel(const GnArgs a) {
     extern __shared__ double sh[];
-    const Where w = where<V>(a);
+    const Where w = where<V>(a, blockIdx.x);
     constexpr int U = 4;
     double s[V], t[V];
 #pragma unroll
@@ -128,26 +164,34 @@ __device__ __forceinline__ double wave_sum(double v) {
     for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o);
     return v;
 }
+// sums of a workgroup of 256 threads, in thread 0
+__device__ __forceinline__ void block_sum2(double& s, double& t) {
+    __shared__ double sh[8];
+    s = wave_sum(s); t = wave_sum(t);
+    if ((threadIdx.x & 63) == 0) { sh[2 * (threadIdx.x >> 6)] = s; sh[2 * (threadIdx.x >> 6) + 1] = t; }
+    __syncthreads();
+    s = (sh[0] + sh[2]) + (sh[4] + sh[6]);
+    t = (sh[1] + sh[3]) + (sh[5] + sh[7]);
+}
+__device__ __forceinline__ void statistics_of(double s, double t, double inv_m, float eps, float& mean, float& rstd) {
+    const double m = s * inv_m;
+    double var = t * inv_m - m * m;
+    if (var < 0.0) var = 0.0;                        // (a constant group; NaN stays NaN)
+    mean = (float)m;
+    rstd = (float)(1.0 / sqrt(var + (double)eps));
+}
 
-// one wave per (sample, group)
-__global__ __launch_bounds__(256) void gn_finalize_kernel(const double* __restrict__ part, int chunks, int units, int per, int groups, double inv_m, float eps,
+// one workgroup per (sample, group)
+__global__ __launch_bounds__(256) void gn_finalize_kernel(const double* __restrict__ part, int chunks, int units, int per, double inv_m, float eps,
                                                           float* __restrict__ mean, float* __restrict__ rstd) {
-    const int i = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (i >= groups) return;
-    const int G = units / per, n = i / G, g = i % G;
+    const int i = blockIdx.x, G = units / per, n = i / G, g = i % G;
     double s = 0.0, t = 0.0;
-    for (int k = lane; k < chunks * per; k += 64) {
+    for (int k = threadIdx.x; k < chunks * per; k += 256) {
         const double* r = part + ((size_t)(n * (size_t)chunks + k / per) * units + g * per + k % per) * 2;
         s += r[0]; t += r[1];
     }
-    s = wave_sum(s); t = wave_sum(t);
-    if (lane == 0) {
-        const double m = s * inv_m;
-        double var = t * inv_m - m * m;
-        if (var < 0.0) var = 0.0;                    // (a constant group; NaN stays NaN)
-        mean[i] = (float)m;
-        rstd[i] = (float)(1.0 / sqrt(var + (double)eps));
-    }
+    block_sum2(s, t);
+    if (threadIdx.x == 0) statistics_of(s, t, inv_m, eps, mean[i], rstd[i]);
 }
 
 // act(z): slope 0 ReLU, (0, 1] LeakyReLU / identity, ACT_SILU z * sigmoid(z)
@@ -157,13 +201,13 @@ template <bool SILU> __device__ __forceinline__ float activate(float z, float sl
 }
 
 template <int V> struct Consts { float mu[V], a[V], b[V]; };
-template <int V> __device__ __forceinline__ Consts<V> constants(const GnArgs& a, int n, int c) {
+template <int V> __device__ __forceinline__ Consts<V> constants(const GnArgs& a, const float* mean, const float* rstd, int c) {      // the sample's statistics
     Consts<V> k;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-        const int g = n * a.G + (c + e) / a.cg;
-        k.mu[e] = a.mean[g];
-        k.a[e] = a.rstd[g] * (a.gamma ? a.gamma[c + e] : 1.f);
+        const int g = (c + e) / a.cg;
+        k.mu[e] = mean[g];
+        k.a[e] = rstd[g] * (a.gamma ? a.gamma[c + e] : 1.f);
         k.b[e] = a.beta ? a.beta[c + e] : 0.f;
     }
     return k;
@@ -171,11 +215,23 @@ template <int V> __device__ __forceinline__ Consts<V> constants(const GnArgs& a,
 
 template <int DT, int V, bool CK, bool SILU, bool KEEP>
 __global__ __launch_bounds__(MAX_T) void gn_apply_kernel(const GnArgs a) {
-    const Where w = where<V>(a);
+    extern __shared__ double sh[];
+    const Where w = where<V>(a, blockIdx.x);
     constexpr int U = 4;
     typedef typename Elem<DT>::T T;
+    const float* mean = a.mean + (size_t)w.n * a.G; const float* rstd = a.rstd + (size_t)w.n * a.G;
+    if (a.rec) {                             // (uniform)
+        merge_records(a.rec + (size_t)w.n * a.rec_chunks * a.rec_units * 2, a.rec_chunks, a.rec_units, a.rec_per, sh);
+        float* st = reinterpret_cast<float*>(sh + 2 * blockDim.x);
+        for (int g = threadIdx.x; g < a.G; g += blockDim.x) {
+            statistics_of(sh[2 * g], sh[2 * g + 1], a.inv_m, a.eps, st[g], st[a.G + g]);
+            if (w.v0 == 0 && w.tile == 0) { a.mean_out[(size_t)w.n * a.G + g] = st[g]; a.rstd_out[(size_t)w.n * a.G + g] = st[a.G + g]; }
+        }
+        __syncthreads();
+        mean = st; rstd = st + a.G;
+    }
     Consts<V> k{};
-    if (w.on) k = constants<V>(a, w.n, w.c);
+    if (w.on) k = constants<V>(a, mean, rstd, w.c);
     // (KEEP: every lane goes round together -- the checkpoint's blocks are 8 lanes)
     for (long long vb = w.v0; vb < w.v1; vb += U * a.R) {
         In<DT, V, CK> in[U]; bool ok[U];
@@ -234,7 +290,7 @@ template <int V> __device__ __forceinline__ ConstsB<V> constants_b(const GnArgs&
 template <int DT, int V, bool CK, bool SILU>
 __global__ __launch_bounds__(MAX_T) void gn_bwd_reduce_kernel(const GnArgs a) {
     extern __shared__ float shf[];
-    const Where w = where<V>(a);
+    const Where w = where<V>(a, blockIdx.x);
     constexpr int U = 2;
     typedef typename Elem<DT>::T T;
     float s[V], t[V];
@@ -272,42 +328,79 @@ __global__ __launch_bounds__(MAX_T) void gn_bwd_reduce_kernel(const GnArgs a) {
     __syncthreads();
     const int first = w.tile * units;
     double* o = a.part + (size_t)(blockIdx.x / a.tiles) * a.C * 2;
-    sum_rows(shf, t2, a.R, units, [&](int u, double x, double y) { if (first + u < a.C) { o[(first + u) * 2] = x; o[(first + u) * 2 + 1] = y; } });
+    double* gs = reinterpret_cast<double*>(shf + ((2 * a.R * units + 1) & ~1));
+    sum_rows(shf, t2, a.R, units, [&](int u, double x, double y) {
+        if (first + u < a.C) {
+            o[(first + u) * 2] = x; o[(first + u) * 2 + 1] = y;
+            if (a.gpart) { const double g = a.gamma ? (double)a.gamma[first + u] : 1.0; gs[2 * u] = g * x; gs[2 * u + 1] = g * y; }
+        }
+    });
+    if (a.gpart) {                           // (one tile: all channels of the sample's chunk are here)
+        __syncthreads();
+        double* p = a.gpart + (size_t)blockIdx.x * a.G * 2;
+        for (int g = threadIdx.x; g < a.G; g += blockDim.x) {
+            double x = 0.0, y = 0.0;
+            for (int e = 0; e < a.cg; ++e) { x += gs[2 * (g * a.cg + e)]; y += gs[2 * (g * a.cg + e) + 1]; }
+            p[2 * g] = x; p[2 * g + 1] = y;
+        }
+    }
 }
 
-// waves [0, N G): m1, m2 of a group; waves [N G, N G + C): dgamma, dbeta of a channel
+// dgamma, dbeta of 16 channels from the channel records of all samples and chunks: thread = (channel, one of blockDim / 16 record rows)
+__device__ __forceinline__ void sum_channels(const double* part, int records, int C, int c0, float* dgamma, float* dbeta, double* sh) {
+    const int c = c0 + (threadIdx.x & 15), rows = blockDim.x / 16;
+    double s = 0.0, t = 0.0;
+    if (c < C)
+        for (int k = threadIdx.x >> 4; k < records; k += 4 * rows) {
+            double2 v[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) { v[u] = make_double2(0.0, 0.0); if (k + u * rows < records) v[u] = *reinterpret_cast<const double2*>(part + ((size_t)(k + u * rows) * C + c) * 2); }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) { s += v[u].x; t += v[u].y; }
+        }
+    sh[threadIdx.x] = s; sh[blockDim.x + threadIdx.x] = t;
+    __syncthreads();
+    sum_rows(sh, sh + blockDim.x, rows, 16, [&](int u, double x, double y) {
+        if (c0 + u < C) { if (dbeta) dbeta[c0 + u] = (float)x; if (dgamma) dgamma[c0 + u] = (float)y; }
+    });
+}
+
+// workgroups [0, N G): m1, m2 of a group; the ones behind them: dgamma, dbeta of 16 channels each
 __global__ __launch_bounds__(256) void gn_bwd_finalize_kernel(const double* __restrict__ part, int N, int chunks, int C, int G, const float* __restrict__ gamma, double inv_m,
                                                               float* __restrict__ m1, float* __restrict__ m2, float* __restrict__ dgamma, float* __restrict__ dbeta) {
-    const int i = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63, cg = C / G;
-    double s = 0.0, t = 0.0;
+    __shared__ double sh[512];
+    const int i = blockIdx.x, cg = C / G;
     if (i < N * G) {
+        double s = 0.0, t = 0.0;
         const int n = i / G, c0 = (i % G) * cg;
-        for (long long k = lane; k < (long long)chunks * cg; k += 64) {
+        for (long long k = threadIdx.x; k < (long long)chunks * cg; k += 256) {
             const int c = c0 + (int)(k % cg);
             const double* r = part + ((size_t)((size_t)n * chunks + k / cg) * C + c) * 2;
             const double g = gamma ? (double)gamma[c] : 1.0;
             s += g * r[0]; t += g * r[1];
         }
-        s = wave_sum(s); t = wave_sum(t);
-        if (lane == 0) { m1[i] = (float)(s * inv_m); m2[i] = (float)(t * inv_m); }
-    } else if (i < N * G + C) {
-        const int c = i - N * G;
-        for (int k = lane; k < N * chunks; k += 64) { const double* r = part + ((size_t)k * C + c) * 2; s += r[0]; t += r[1]; }
-        s = wave_sum(s); t = wave_sum(t);
-        if (lane == 0) { if (dbeta) dbeta[c] = (float)s; if (dgamma) dgamma[c] = (float)t; }
-    }
+        block_sum2(s, t);
+        if (threadIdx.x == 0) { m1[i] = (float)(s * inv_m); m2[i] = (float)(t * inv_m); }
+    } else sum_channels(part, N * chunks, C, (i - N * G) * 16, dgamma, dbeta, sh);
 }
 
 template <int DT, int V, bool CK, bool SILU>
 __global__ __launch_bounds__(MAX_T) void gn_bwd_apply_kernel(const GnArgs a) {
-    const Where w = where<V>(a);
+    extern __shared__ double sh[];
+    if (blockIdx.x < a.sum_wgs) { sum_channels(a.cpart, a.N * a.rec_chunks, a.C, blockIdx.x * 16, a.dgamma, a.dbeta, sh); return; }
+    const Where w = where<V>(a, blockIdx.x - a.sum_wgs);
     constexpr int U = 2;
     typedef typename Elem<DT>::T T;
+    float m1[V], m2[V];
+    if (a.rec) merge_records(a.rec + (size_t)w.n * a.rec_chunks * a.rec_units * 2, a.rec_chunks, a.rec_units, a.rec_per, sh);
     if (!w.on) return;
     const ConstsB<V> k = constants_b<V>(a, w.n, w.c);
-    float m1[V], m2[V];
 #pragma unroll
-    for (int e = 0; e < V; ++e) { const int g = w.n * a.G + (w.c + e) / a.cg; m1[e] = a.m1[g]; m2[e] = a.m2[g]; }
+    for (int e = 0; e < V; ++e) {
+        const int g = (w.c + e) / a.cg;
+        if (a.rec) { m1[e] = (float)(sh[2 * g] * a.inv_m); m2[e] = (float)(sh[2 * g + 1] * a.inv_m); }
+        else { m1[e] = a.m1[w.n * a.G + g]; m2[e] = a.m2[w.n * a.G + g]; }
+    }
     for (long long v = w.v0 + w.r; v < w.v1; v += U * a.R) {
         In<DT, V, CK> in[U]; Raw<DT, V> dy[U]; bool ok[U];
 #pragma unroll
@@ -359,7 +452,11 @@ template <int V> void map_pass(GnArgs& a, const Shape& sh, int target, int U, bo
 dim3 grid_of(const GnArgs& a) { return dim3((unsigned)((long long)a.N * a.chunks * a.tiles)); }
 dim3 block_of(const GnArgs& a) { return dim3((unsigned)((a.R * a.PT + 63) / 64 * 64)); }
 
-constexpr int STATS_WGS = 2048, APPLY_WGS = 2048;
+#ifndef GN_STATS_WGS
+#define GN_STATS_WGS 512
+#define GN_APPLY_WGS 1024
+#endif
+constexpr int STATS_WGS = GN_STATS_WGS, APPLY_WGS = GN_APPLY_WGS;
 
 template <int V> int unit_of(int cg) {
     int u = V;
@@ -371,26 +468,34 @@ template <int V> size_t fwd_part_doubles(const Shape& sh) {
     GnArgs a{}; map_pass<V>(a, sh, STATS_WGS, 4, false);
     return (size_t)sh.N * a.chunks * (sh.C / unit_of<V>(sh.C / sh.G)) * 2;
 }
-template <int V> size_t bwd_part_doubles(const Shape& sh) {
-    GnArgs a{}; map_pass<V>(a, sh, STATS_WGS, 2, false);
-    return (size_t)sh.N * a.chunks * sh.C * 2;
+// what lies in the workspace of a backward pass: channel records, then group records (`merge`) or m1 and m2
+struct BwdSpace { size_t channels, behind; bool merge; };
+template <int V> BwdSpace bwd_space(const GnArgs& a, const Shape& sh) {
+    BwdSpace b;
+    b.merge = a.tiles == 1 && sh.C <= 1024 && sh.G <= MERGE_UNITS && (long long)a.chunks * sh.G <= MERGE_MAX;
+    b.channels = align_up((size_t)sh.N * a.chunks * sh.C * 2 * sizeof(double), 256);
+    b.behind = b.merge ? (size_t)sh.N * a.chunks * sh.G * 2 * sizeof(double) : (size_t)2 * sh.N * sh.G * sizeof(float);
+    return b;
 }
 size_t max2(size_t a, size_t b) { return a > b ? a : b; }
-size_t workspace_bytes(const Shape& sh) {
-    size_t d = max2(fwd_part_doubles<1>(sh), bwd_part_doubles<1>(sh));
-    if (sh.C % 8 == 0) d = max2(d, max2(fwd_part_doubles<8>(sh), bwd_part_doubles<8>(sh)));
-    return align_up(d * sizeof(double), 256) + align_up((size_t)2 * sh.N * sh.G * sizeof(float), 256);
+template <int V> size_t space_of(const Shape& sh) {
+    GnArgs a{}; map_pass<V>(a, sh, STATS_WGS, 2, false);
+    const BwdSpace b = bwd_space<V>(a, sh);
+    return max2(fwd_part_doubles<V>(sh) * sizeof(double), b.channels + b.behind);
 }
+size_t workspace_bytes(const Shape& sh) { return max2(space_of<1>(sh), sh.C % 8 == 0 ? space_of<8>(sh) : 0); }
+size_t merge_lds(const GnArgs& a, int units) { return (size_t)2 * (block_of(a).x + units) * sizeof(double); }
 
 template <int DT, int V, bool CK> void launch_apply(GnArgs a, const Shape& sh, hipStream_t s) {
     const bool keep = a.q_out != nullptr;
     map_pass<V>(a, sh, APPLY_WGS, 4, keep);
+    const size_t lds = a.rec ? merge_lds(a, a.rec_units) : 0;
     if (a.slope == ACT_SILU) {
-        if constexpr (V == 8 && !CK) if (keep) { hipLaunchKernelGGL((gn_apply_kernel<DT, V, CK, true, true>), grid_of(a), block_of(a), 0, s, a); return; }
-        hipLaunchKernelGGL((gn_apply_kernel<DT, V, CK, true, false>), grid_of(a), block_of(a), 0, s, a);
+        if constexpr (V == 8 && !CK) if (keep) { hipLaunchKernelGGL((gn_apply_kernel<DT, V, CK, true, true>), grid_of(a), block_of(a), lds, s, a); return; }
+        hipLaunchKernelGGL((gn_apply_kernel<DT, V, CK, true, false>), grid_of(a), block_of(a), lds, s, a);
     } else {
-        if constexpr (V == 8 && !CK) if (keep) { hipLaunchKernelGGL((gn_apply_kernel<DT, V, CK, false, true>), grid_of(a), block_of(a), 0, s, a); return; }
-        hipLaunchKernelGGL((gn_apply_kernel<DT, V, CK, false, false>), grid_of(a), block_of(a), 0, s, a);
+        if constexpr (V == 8 && !CK) if (keep) { hipLaunchKernelGGL((gn_apply_kernel<DT, V, CK, false, true>), grid_of(a), block_of(a), lds, s, a); return; }
+        hipLaunchKernelGGL((gn_apply_kernel<DT, V, CK, false, false>), grid_of(a), block_of(a), lds, s, a);
     }
 }
 
@@ -401,9 +506,13 @@ template <int DT, int V> int forward(GnArgs a, const Shape& sh, float eps, float
     st.part = (double*)ws;
     const int units = sh.C / st.unit;
     hipLaunchKernelGGL((gn_stats_kernel<DT, V>), grid_of(st), block_of(st), (size_t)st.R * st.PT * (V / st.unit) * 2 * sizeof(double), s, st);
-    hipLaunchKernelGGL(gn_finalize_kernel, dim3((sh.N * sh.G + 3) / 4), dim3(256), 0, s, st.part, st.chunks, units, st.cg / st.unit, sh.N * sh.G,
-                       1.0 / ((double)sh.S * st.cg), eps, mean, rstd);
+    const double inv_m = 1.0 / ((double)sh.S * st.cg);
     a.mean = mean; a.rstd = rstd;
+    if ((long long)st.chunks * units <= MERGE_MAX && units <= MERGE_UNITS) {
+        a.rec = st.part; a.rec_chunks = st.chunks; a.rec_units = units; a.rec_per = st.cg / st.unit;
+        a.inv_m = inv_m; a.eps = eps; a.mean_out = mean; a.rstd_out = rstd;
+    } else
+        hipLaunchKernelGGL(gn_finalize_kernel, dim3(sh.N * sh.G), dim3(256), 0, s, st.part, st.chunks, units, st.cg / st.unit, inv_m, eps, mean, rstd);
     // the checkpoint rides in the apply pass where its blocks are whole there; otherwise it is a pass of its own
     signed char* q = a.q_out; float* qs = a.qs_out;
     GnArgs m{}; map_pass<V>(m, sh, APPLY_WGS, 4, true);
@@ -419,17 +528,30 @@ template <int DT, int V, bool CK> int backward(GnArgs a, const Shape& sh, float*
     GnArgs st = a;
     map_pass<V>(st, sh, STATS_WGS, 2, false);
     st.part = (double*)ws;
-    float* m1 = (float*)((char*)ws + align_up((size_t)sh.N * st.chunks * sh.C * 2 * sizeof(double), 256));
-    float* m2 = m1 + (size_t)sh.N * sh.G;
-    const size_t lds = (size_t)st.R * st.PT * V * 2 * sizeof(float);
+    const BwdSpace space = bwd_space<V>(st, sh);
+    void* behind = (char*)ws + space.channels;
+    const bool merge = space.merge;
+    if (merge) st.gpart = (double*)behind;
+    const size_t lds = align_up((size_t)st.R * st.PT * V * 2 * sizeof(float), 8) + (merge ? (size_t)sh.C * 2 * sizeof(double) : 0);
     if (a.slope == ACT_SILU) hipLaunchKernelGGL((gn_bwd_reduce_kernel<DT, V, CK, true>), grid_of(st), block_of(st), lds, s, st);
     else hipLaunchKernelGGL((gn_bwd_reduce_kernel<DT, V, CK, false>), grid_of(st), block_of(st), lds, s, st);
-    hipLaunchKernelGGL(gn_bwd_finalize_kernel, dim3((sh.N * sh.G + sh.C + 3) / 4), dim3(256), 0, s, st.part, sh.N, st.chunks, sh.C, sh.G, a.gamma,
-                       1.0 / ((double)sh.S * st.cg), m1, m2, dgamma, dbeta);
     map_pass<V>(a, sh, APPLY_WGS, 2, false);
-    a.m1 = m1; a.m2 = m2;
-    if (a.slope == ACT_SILU) hipLaunchKernelGGL((gn_bwd_apply_kernel<DT, V, CK, true>), grid_of(a), block_of(a), 0, s, a);
-    else hipLaunchKernelGGL((gn_bwd_apply_kernel<DT, V, CK, false>), grid_of(a), block_of(a), 0, s, a);
+    a.inv_m = 1.0 / ((double)sh.S * st.cg);
+    size_t alds = 0;
+    const int sums = (dgamma || dbeta) ? (sh.C + 15) / 16 : 0;
+    if (merge) {
+        a.rec = st.gpart; a.rec_chunks = st.chunks; a.rec_units = sh.G; a.rec_per = 1;
+        a.cpart = st.part; a.dgamma = dgamma; a.dbeta = dbeta; a.sum_wgs = sums;
+        alds = merge_lds(a, sh.G);
+    } else {
+        float* m1 = (float*)behind;
+        float* m2 = m1 + (size_t)sh.N * sh.G;
+        hipLaunchKernelGGL(gn_bwd_finalize_kernel, dim3(sh.N * sh.G + sums), dim3(256), 0, s, st.part, sh.N, st.chunks, sh.C, sh.G, a.gamma, a.inv_m, m1, m2, dgamma, dbeta);
+        a.m1 = m1; a.m2 = m2;
+    }
+    const dim3 grid(grid_of(a).x + a.sum_wgs);
+    if (a.slope == ACT_SILU) hipLaunchKernelGGL((gn_bwd_apply_kernel<DT, V, CK, true>), grid, block_of(a), alds, s, a);
+    else hipLaunchKernelGGL((gn_bwd_apply_kernel<DT, V, CK, false>), grid, block_of(a), alds, s, a);
     E3_CHECK_HIP(hipGetLastError());
     return E3_OK;
 }
