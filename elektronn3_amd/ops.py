@@ -330,60 +330,68 @@ def convT_wgrad_bf16(x, dy):
 
 
 # ------------------------------------------------------------------ group norm with an activation, 8-bit activation checkpoints
+# (small calls are bound by this file: a forward is two launches of 4 us, so the checks below look at every property once and tensors are allocated once)
 _DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}       # E3_DT_*
+_SLOPES = {'relu': 0.0, 'leaky': 0.1, 'lin': 1.0, 'silu': 2.0}
+_raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def _chk_any(t, name, like=None):
-    """An fp32 / bf16 / fp16 NDHWC view on a ROCm device (with the shape, type and device of `like`)."""
+def _call(device, fn, *args):
+    """One native call on the tensors' device and its current stream."""
+    if torch.cuda.current_device() == device.index:
+        rc = fn(_raw_stream(device.index), *args)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(_raw_stream(device.index), *args)
+    if rc:
+        check(rc)
+
+
+def _chk_any(t, name, shape=None, dtype=None, device=None):
+    """Row length of an fp32 / bf16 / fp16 NDHWC view on a ROCm device (with the given shape, type and device)."""
     if not isinstance(t, torch.Tensor) or t.dtype not in _DT:
         raise ValueError(f'{name}: expected a float32, bfloat16 or float16 tensor')
     if not t.is_cuda:
         raise ValueError(f'{name}: expected a CUDA tensor (the HIP path has no CPU fallback)')
+    if shape is not None and (t.shape != shape or t.dtype != dtype or t.device != device):
+        raise ValueError(f'{name}: expected shape {tuple(shape)}, {dtype} on {device}, got {tuple(t.shape)}, {t.dtype} on {t.device}')
     if t.dim() != 5:
         raise ValueError(f'{name}: expected a 5D (N, D, H, W, C) tensor, got {t.dim()}D')
-    if like is not None and (tuple(t.shape) != tuple(like.shape) or t.dtype != like.dtype or t.device != like.device):
-        raise ValueError(f'{name}: expected shape {tuple(like.shape)}, {like.dtype} on {like.device}, got {tuple(t.shape)}, {t.dtype} on {t.device}')
-    return _ldc(t) if t.numel() else max(t.shape[4], 1)
+    return t.shape[4] or 1 if t.is_contiguous() else _ldc(t)
 
 
-def _chk_out(out, ins, name='out'):
-    """`out` may be one of the inputs itself (the same view); a view that overlaps one otherwise would be read after it was written."""
-    lo = out.data_ptr()
-    hi = lo + ((out.shape[0] - 1) * out.stride(0) + (out.shape[1] - 1) * out.stride(1) + (out.shape[2] - 1) * out.stride(2)
-               + (out.shape[3] - 1) * out.stride(3) + out.shape[4]) * out.element_size() if out.numel() else lo
-    for t in ins:
-        if t is None or t.numel() == 0 or (t.data_ptr() == lo and t.dtype == out.dtype and t.stride() == out.stride()):
-            continue
-        a = t.data_ptr()
-        b = a + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
-        # (the two halves of a concat buffer interleave in memory without sharing an element: rows of the same buffer, other channels)
-        if a < hi and lo < b and not _disjoint_channels(t, out):
-            raise ValueError(f'{name} overlaps an input without being the same view')
+def _span(t):
+    lo = t.data_ptr()
+    return lo, lo + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
 
 
-def _disjoint_channels(t, out):
-    if t.dtype != out.dtype or t.dim() != 5:
-        return False
-    ldc, d = _ldc(out), (t.data_ptr() - out.data_ptr())
-    if _ldc(t) != ldc or d % t.element_size():
-        return False
-    d = (d // t.element_size()) % ldc
-    return d >= out.shape[4] and d + t.shape[4] <= ldc
+def _chk_out(out, t, name='out'):
+    """`out` may be the input itself (the same view); a view that overlaps it otherwise would be read after it was written."""
+    if out.numel() == 0 or (t.data_ptr() == out.data_ptr() and t.stride() == out.stride()):
+        return
+    (a, b), (c, d) = _span(t), _span(out)
+    if a < d and c < b:
+        # (halves of one concat buffer interleave in memory without sharing an element: rows of the same length, other channels)
+        ldc, size = _ldc(out), out.element_size()
+        off = (a - c) // size % ldc
+        if _ldc(t) != ldc or (a - c) % size or off < out.shape[4] or off + t.shape[4] > ldc:
+            raise ValueError(f'{name} overlaps the input without being the same view')
 
 
 def _chk_vec(t, n, name, device):
-    if t is None:
-        return None
     if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.numel() != n or t.device != device:
         raise ValueError(f'{name}: expected {n} float32 values on {device}')
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _act_slope(activation):
     """Slope code of the C ABI from an activation's name or module (those of UNet(activation=...)); nn.PReLU and nn.RReLU are not covered."""
-    from .unet import _activation_slope
-    slope = _activation_slope(activation)
-    if slope is None or slope == 3.0 or activation == 'rrelu' or isinstance(activation, torch.nn.RReLU):
+    if isinstance(activation, str):
+        slope = _SLOPES.get(activation)
+    else:
+        from .unet import _activation_slope
+        slope = _activation_slope(activation)
+    if slope is None or slope == 3.0 or isinstance(activation, torch.nn.RReLU):
         raise NotImplementedError(f"activation {activation!r}: 'relu', 'leaky', 'lin', 'silu' or their modules")
     return slope
 
@@ -393,10 +401,10 @@ class Checkpoint8:
     elements).  It stands for ``q * scale`` (3.76 times smaller than float32, 1.88 times than a 16-bit type); an element is off by at most half
     a step, ``amax / 254`` of its block's largest magnitude.  A block with a NaN or an infinity stands for NaNs.  Made by :func:`checkpoint8` or
     :func:`group_norm_act`; read by :func:`checkpoint8_restore`, :func:`group_norm_act_apply` and :func:`group_norm_act_bwd`."""
-    __slots__ = ('q', 'scale', 'shape', 'dtype')
+    __slots__ = ('q', 'scale', 'shape', 'dtype', 'device')
 
     def __init__(self, q, scale, shape, dtype):
-        shape = torch.Size(int(s) for s in shape)
+        shape = torch.Size(shape)
         n = shape.numel()
         if len(shape) != 5 or dtype not in _DT:
             raise ValueError('Checkpoint8: expected the (N, D, H, W, C) shape and the float32, bfloat16 or float16 type of the tensor it stands for')
@@ -406,11 +414,7 @@ class Checkpoint8:
             raise ValueError(f'Checkpoint8: scale: expected {-(-n // 64)} contiguous float32 values on {q.device}')
         if not q.is_cuda:
             raise ValueError('Checkpoint8: expected CUDA tensors (the HIP path has no CPU fallback)')
-        self.q, self.scale, self.shape, self.dtype = q, scale, shape, dtype
-
-    @property
-    def device(self):
-        return self.q.device
+        self.q, self.scale, self.shape, self.dtype, self.device = q, scale, shape, dtype, q.device
 
     @property
     def nbytes(self):
@@ -425,15 +429,18 @@ class Checkpoint8:
 
 def _new_checkpoint(x):
     n = x.numel()
-    return Checkpoint8(torch.empty(n, dtype=torch.int8, device=x.device), torch.empty(-(-n // 64), dtype=torch.float32, device=x.device), x.shape, x.dtype)
+    ck = Checkpoint8.__new__(Checkpoint8)
+    ck.q, ck.scale = torch.empty(n, dtype=torch.int8, device=x.device), torch.empty(-(-n // 64), dtype=torch.float32, device=x.device)
+    ck.shape, ck.dtype, ck.device = x.shape, x.dtype, x.device
+    return ck
 
 
 def checkpoint8(x):
     """Keeps an activation (float32 / bfloat16 / float16 NDHWC view) in 8 bits; see :class:`Checkpoint8`."""
     ldc = _chk_any(x, 'x')
     ck = _new_checkpoint(x)
-    with torch.cuda.device(x.device):
-        check(_lib.load().e3_checkpoint8_pack(stream_ptr(x.device), _DT[x.dtype], ptr(x), ldc, x.numel() // max(x.shape[4], 1), x.shape[4] or 1, ptr(ck.q), ptr(ck.scale)))
+    C = x.shape[4] or 1
+    _call(ck.device, _lib.load().e3_checkpoint8_pack, _DT[x.dtype], x.data_ptr(), ldc, x.numel() // C, C, ck.q.data_ptr(), ck.scale.data_ptr())
     return ck
 
 
@@ -441,35 +448,46 @@ def checkpoint8_restore(ck, out=None):
     """The tensor that a :class:`Checkpoint8` stands for, rounded to its type (into ``out``, an NDHWC view, if given)."""
     if not isinstance(ck, Checkpoint8):
         raise ValueError('expected a Checkpoint8')
-    y = out if out is not None else torch.empty(ck.shape, dtype=ck.dtype, device=ck.device)
-    ldc = _chk_any(y, 'out', like=ck)
-    with torch.cuda.device(ck.device):
-        check(_lib.load().e3_checkpoint8_unpack(stream_ptr(ck.device), _DT[ck.dtype], ptr(ck.q), ptr(ck.scale), ck.numel() // max(ck.shape[4], 1), ck.shape[4] or 1,
-                                                ptr(y), ldc))
-    return y
+    C = ck.shape[4] or 1
+    if out is None:
+        out, ldc = torch.empty(ck.shape, dtype=ck.dtype, device=ck.device), C
+    else:
+        ldc = _chk_any(out, 'out', ck.shape, ck.dtype, ck.device)
+    _call(ck.device, _lib.load().e3_checkpoint8_unpack, _DT[ck.dtype], ck.q.data_ptr(), ck.scale.data_ptr(), ck.q.numel() // C, C, out.data_ptr(), ldc)
+    return out
 
 
 def _source(x):
     """(x pointer, ldc, q pointer, scale pointer) of a tensor or a checkpoint of it."""
     if isinstance(x, Checkpoint8):
-        return None, 0, ptr(x.q), ptr(x.scale)
-    return ptr(x), _chk_any(x, 'x'), None, None
+        return None, 0, x.q.data_ptr(), x.scale.data_ptr()
+    ldc = _chk_any(x, 'x')
+    return x.data_ptr(), ldc, None, None
 
 
-def _gn_dims(x, num_groups):
-    N, D, H, W, C = x.shape
-    if min(x.shape) < 1:
-        raise ValueError(f'x: expected at least one element, got shape {tuple(x.shape)}')
+def _gn_dims(shape, num_groups):
+    N, D, H, W, C = shape
+    if N < 1 or D < 1 or H < 1 or W < 1 or C < 1:
+        raise ValueError(f'x: expected at least one element, got shape {tuple(shape)}')
     if num_groups < 1 or C % num_groups != 0:
         raise ValueError('num_channels must be divisible by num_groups')
     return N, D, H, W, C, num_groups
 
 
-def _stats(x, mean, rstd):
-    if mean.dim() != 2 or mean.shape[0] != x.shape[0]:
-        raise ValueError(f'mean: expected shape ({x.shape[0]}, num_groups)')
+def _affine(weight, bias, C, device):
+    """(tensors to keep alive, pointers) of the norm's parameters"""
+    if weight is not None:
+        weight = _chk_vec(weight, C, 'weight', device)
+    if bias is not None:
+        bias = _chk_vec(bias, C, 'bias', device)
+    return weight, bias, weight.data_ptr() if weight is not None else None, bias.data_ptr() if bias is not None else None
+
+
+def _stats(mean, rstd, N, device):
+    if not isinstance(mean, torch.Tensor) or mean.dim() != 2 or mean.shape[0] != N:
+        raise ValueError(f'mean: expected shape ({N}, num_groups)')
     n = mean.numel()
-    return _chk_vec(mean, n, 'mean', x.device), _chk_vec(rstd, n, 'rstd', x.device), mean.shape[1]
+    return _chk_vec(mean, n, 'mean', device), _chk_vec(rstd, n, 'rstd', device), mean.shape[1]
 
 
 def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, activation='relu', checkpoint=False, out=None):
@@ -478,38 +496,45 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, activation='
     ``(y, mean, rstd, Checkpoint8)``.  ``out`` may be ``x`` itself."""
     slope = _act_slope(activation)
     ldc = _chk_any(x, 'x')
-    dims = _gn_dims(x, num_groups)
-    weight, bias = _chk_vec(weight, x.shape[4], 'weight', x.device), _chk_vec(bias, x.shape[4], 'bias', x.device)
+    shape, dtype, device = x.shape, x.dtype, x.device
+    dims = _gn_dims(shape, num_groups)
+    C = dims[4]
+    weight, bias, wp, bp = _affine(weight, bias, C, device)
     if not eps >= 0:
         raise ValueError('eps must not be negative')
-    y = out if out is not None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    y_ldc = _chk_any(y, 'out', like=x)
-    if out is not None:
-        _chk_out(out, (x,))
+    if out is None:
+        y, y_ldc = torch.empty(shape, dtype=dtype, device=device), C
+    else:
+        y, y_ldc = out, _chk_any(out, 'out', shape, dtype, device)
+        _chk_out(out, x)
     L = _lib.load()
-    mean, rstd = (torch.empty((x.shape[0], num_groups), dtype=torch.float32, device=x.device) for _ in range(2))
+    mean = torch.empty((dims[0], num_groups), dtype=torch.float32, device=device)
+    rstd = torch.empty((dims[0], num_groups), dtype=torch.float32, device=device)
     ck = _new_checkpoint(x) if checkpoint else None
-    ws = _ws(L.e3_group_norm_workspace_bytes(*dims), x.device)
-    with torch.cuda.device(x.device):
-        check(L.e3_group_norm_act_fwd(stream_ptr(x.device), _DT[x.dtype], ptr(x), ldc, ptr(weight), ptr(bias), float(eps), slope, ptr(y), y_ldc, ptr(mean), ptr(rstd),
-                                      ptr(ck.q) if ck else None, ptr(ck.scale) if ck else None, *dims, ptr(ws), c_size_t(ws.numel())))
+    nbytes = L.e3_group_norm_workspace_bytes(*dims)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    _call(device, L.e3_group_norm_act_fwd, _DT[dtype], x.data_ptr(), ldc, wp, bp, eps, slope, y.data_ptr(), y_ldc, mean.data_ptr(), rstd.data_ptr(),
+          ck.q.data_ptr() if ck else None, ck.scale.data_ptr() if ck else None, *dims, ws.data_ptr(), nbytes)
     return (y, mean, rstd, ck) if checkpoint else (y, mean, rstd)
 
 
 def group_norm_act_apply(x, mean, rstd, weight=None, bias=None, activation='relu', out=None):
     """``y`` of :func:`group_norm_act` from its statistics and its input or the input's :class:`Checkpoint8` (the activation recomputed in a backward
-    pass; a checkpoint's values enter in float32)."""
+    pass; a checkpoint's values enter in float32).  ``out`` may be ``x`` itself."""
     slope = _act_slope(activation)
     src = _source(x)
-    mean, rstd, G = _stats(x, mean, rstd)
-    dims = _gn_dims(x, G)
-    weight, bias = _chk_vec(weight, x.shape[4], 'weight', x.device), _chk_vec(bias, x.shape[4], 'bias', x.device)
-    y = out if out is not None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    y_ldc = _chk_any(y, 'out', like=x)
-    if out is not None and not isinstance(x, Checkpoint8):
-        _chk_out(out, (x,))
-    with torch.cuda.device(x.device):
-        check(_lib.load().e3_group_norm_act_apply(stream_ptr(x.device), _DT[x.dtype], *src, ptr(mean), ptr(rstd), ptr(weight), ptr(bias), slope, ptr(y), y_ldc, *dims))
+    shape, dtype, device = x.shape, x.dtype, x.device
+    mean, rstd, G = _stats(mean, rstd, shape[0], device)
+    dims = _gn_dims(shape, G)
+    C = dims[4]
+    weight, bias, wp, bp = _affine(weight, bias, C, device)
+    if out is None:
+        y, y_ldc = torch.empty(shape, dtype=dtype, device=device), C
+    else:
+        y, y_ldc = out, _chk_any(out, 'out', shape, dtype, device)
+        if src[0] is not None:
+            _chk_out(out, x)
+    _call(device, _lib.load().e3_group_norm_act_apply, _DT[dtype], *src, mean.data_ptr(), rstd.data_ptr(), wp, bp, slope, y.data_ptr(), y_ldc, *dims)
     return y
 
 
@@ -518,16 +543,18 @@ def group_norm_act_bwd(x, mean, rstd, dy, weight=None, bias=None, activation='re
     dbias are float32 (C,) whether or not the norm has parameters."""
     slope = _act_slope(activation)
     src = _source(x)
-    mean, rstd, G = _stats(x, mean, rstd)
-    dims = _gn_dims(x, G)
-    C = x.shape[4]
-    weight, bias = _chk_vec(weight, C, 'weight', x.device), _chk_vec(bias, C, 'bias', x.device)
-    dy_ldc = _chk_any(dy, 'dy', like=x)
+    shape, dtype, device = x.shape, x.dtype, x.device
+    mean, rstd, G = _stats(mean, rstd, shape[0], device)
+    dims = _gn_dims(shape, G)
+    C = dims[4]
+    weight, bias, wp, bp = _affine(weight, bias, C, device)
+    dy_ldc = _chk_any(dy, 'dy', shape, dtype, device)
     L = _lib.load()
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    dw, db = (torch.empty(C, dtype=torch.float32, device=x.device) for _ in range(2))
-    ws = _ws(L.e3_group_norm_workspace_bytes(*dims), x.device)
-    with torch.cuda.device(x.device):
-        check(L.e3_group_norm_act_bwd(stream_ptr(x.device), _DT[x.dtype], *src, ptr(mean), ptr(rstd), ptr(weight), ptr(bias), slope, ptr(dy), dy_ldc, ptr(dx), C,
-                                      ptr(dw), ptr(db), *dims, ptr(ws), c_size_t(ws.numel())))
+    dx = torch.empty(shape, dtype=dtype, device=device)
+    dw = torch.empty(C, dtype=torch.float32, device=device)
+    db = torch.empty(C, dtype=torch.float32, device=device)
+    nbytes = L.e3_group_norm_workspace_bytes(*dims)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    _call(device, L.e3_group_norm_act_bwd, _DT[dtype], *src, mean.data_ptr(), rstd.data_ptr(), wp, bp, slope, dy.data_ptr(), dy_ldc, dx.data_ptr(), C,
+          dw.data_ptr(), db.data_ptr(), *dims, ws.data_ptr(), nbytes)
     return dx, dw, db
