@@ -7,12 +7,15 @@
 //
 // All kernels are streaming passes with one mapping: a thread keeps V consecutive channels (V = 8: 16-byte accesses; V = 1 for rows that do not allow them) and
 // walks the voxels of its workgroup's chunk, so that the per-channel constants stay in registers; consecutive threads take consecutive pieces of a voxel, then
-// consecutive voxels.  A workgroup works on one chunk of one sample and, for more than 512 pieces per voxel, on one tile of its channels.
+// consecutive voxels.  A workgroup works on one chunk of one sample and, for more than 512 pieces per voxel, on one tile of its channels.  UN is the number of
+// consecutive channels of a piece that surely share a group (8, 4 or 1): V / UN constants or sums per thread instead of V, which decides the register count.
 //   forward:   statistics (read x) -> apply (read x, write y [, write the checkpoint])
 //   backward:  reduce (read x, dy) -> apply (read x, dy, write dx)
 // Sums leave a workgroup as fp64 records [sample][chunk][..], merged in a fixed order: results do not depend on timing.  Every workgroup of the apply pass
 // merges its sample's records itself (a few tens of KB out of L2, about 1 us) instead of waiting for a third launch in between; where the records of a
 // sample are more than MERGE_MAX a finalising launch does it.
+#include <type_traits>
+
 #include "checkpoint8.h"
 
 #include "../../include/e3unet.h"
@@ -36,8 +39,7 @@ struct GnArgs {
     int N, C, G, cg; long long S;
     int P, PT, tiles, R;                     // pieces per voxel, pieces per tile, tiles, voxels per workgroup step
     int chunks; long long chunk;             // chunks of a sample, voxels of a chunk
-    int unit;                                // channels that the statistics pass adds up before it writes them (divides cg and V)
-    double* part;                            // records (sum, sum of squares) [N][chunks][C / unit] | (sum dz, sum dz h) [N][chunks][C]
+    double* part;                            // records (sum, sum of squares) [N][chunks][C / UN] | (sum dz, sum dz h) [N][chunks][C]
     double* gpart;                           // backward: (sum gamma dz, sum gamma dz h) [N][chunks][G], or nullptr
     // apply passes that merge the records themselves (rec != nullptr)
     const double* rec; int rec_chunks, rec_units, rec_per;      // [N][rec_chunks][rec_units] pairs, rec_per units to a group
@@ -73,6 +75,12 @@ template <int DT, int V> struct In<DT, V, true> {
     __device__ __forceinline__ void load(const GnArgs& a, long long row, int c) { r = load_q<V>(a.q, a.qs, (size_t)row * a.C + c); }
     __device__ __forceinline__ void get(float (&f)[V]) const { unpack_q<V>(r, f); }
 };
+
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
 
 // Sums of `rows` x `units` pairs in LDS over the rows: L lanes share a unit (fixed order), lane 0 hands the sums on.
 template <typename T, typename F> __device__ __forceinline__ void sum_rows(const T* a, const T* b, int rows, int units, F done) {
@@ -117,53 +125,14 @@ __device__ __forceinline__ void merge_records(const double* rec, int chunks, int
 constexpr int MERGE_MAX = 4096;              // records of a sample that the apply pass merges itself (64 KB)
 constexpr int MERGE_UNITS = 128;             // ... of at most so many units (a workgroup has 192 threads or more)
 
-// ------------------------------------------------------------------------------------------------ forward
-// Sums and sums of squares in fp64: the variance is then a difference that loses nothing an fp32 input holds, whatever its mean.
-template <int DT, int V>
-__global__ __launch_bounds__(MAX_T) void gn_stats_kernel(const GnArgs a) {
-    extern __shared__ double sh[];
-    const Where w = where<V>(a, blockIdx.x);
-    constexpr int U = 4;
-    double s[V], t[V];
-#pragma unroll
-    for (int e = 0; e < V; ++e) s[e] = t[e] = 0.0;
-    if (w.on)
-        for (long long v = w.v0 + w.r; v < w.v1; v += U * a.R) {
-            In<DT, V, false> in[U]; bool ok[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) { ok[u] = v + u * a.R < w.v1; in[u].r = Raw<DT, V>{}; if (ok[u]) in[u].load(a, w.n * a.S + v + u * a.R, w.c); }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                float f[V];
-                in[u].get(f);
-#pragma unroll
-                for (int e = 0; e < V; ++e) { const double d = f[e]; s[e] += d; t[e] = fma(d, d, t[e]); }      // (a piece that is not there is zeros)
-            }
-        }
-    // channels of one unit are added up in the thread (all of them belong to one group), then the rows of the workgroup
-#pragma unroll
-    for (int k = 1; k < V; k <<= 1)
-        if (a.unit > k)
-#pragma unroll
-            for (int e = 0; e < V; e += 2 * k) { s[e] += s[e + k]; t[e] += t[e + k]; }
-    const int K = V / a.unit, units = a.PT * K;
-    double* s2 = sh + a.R * units;
-    if (w.r < a.R) {
-#pragma unroll
-        for (int e = 0; e < V; ++e)
-            if (e % a.unit == 0) { const int i = w.r * units + (int)(threadIdx.x % a.PT) * K + e / a.unit; sh[i] = s[e]; s2[i] = t[e]; }
-    }
-    __syncthreads();
-    const int all = a.C / a.unit, first = w.tile * units;
-    double* o = a.part + (size_t)(blockIdx.x / a.tiles) * all * 2;
-    sum_rows(sh, s2, a.R, units, [&](int u, double x, double y) { if (first + u < all) { o[(first + u) * 2] = x; o[(first + u) * 2 + 1] = y; } });
+__device__ __forceinline__ void statistics_of(double s, double t, double inv_m, float eps, float& mean, float& rstd) {
+    const double m = s * inv_m;
+    double var = t * inv_m - m * m;
+    if (var < 0.0) var = 0.0;                        // (a constant group; NaN stays NaN)
+    mean = (float)m;
+    rstd = (float)(1.0 / sqrt(var + (double)eps));
 }
 
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o);
-    return v;
-}
 // sums of a workgroup of 256 threads, in thread 0
 __device__ __forceinline__ void block_sum2(double& s, double& t) {
     __shared__ double sh[8];
@@ -172,13 +141,6 @@ __device__ __forceinline__ void block_sum2(double& s, double& t) {
     __syncthreads();
     s = (sh[0] + sh[2]) + (sh[4] + sh[6]);
     t = (sh[1] + sh[3]) + (sh[5] + sh[7]);
-}
-__device__ __forceinline__ void statistics_of(double s, double t, double inv_m, float eps, float& mean, float& rstd) {
-    const double m = s * inv_m;
-    double var = t * inv_m - m * m;
-    if (var < 0.0) var = 0.0;                        // (a constant group; NaN stays NaN)
-    mean = (float)m;
-    rstd = (float)(1.0 / sqrt(var + (double)eps));
 }
 
 // one workgroup per (sample, group)
@@ -194,26 +156,67 @@ __global__ __launch_bounds__(256) void gn_finalize_kernel(const double* __restri
     if (threadIdx.x == 0) statistics_of(s, t, inv_m, eps, mean[i], rstd[i]);
 }
 
+// the constants of a piece: a = rstd gamma
+template <int V, int UN> struct Consts { float mu[V / UN], rs[V / UN], a[V], b[V]; };
+template <int V, int UN> __device__ __forceinline__ Consts<V, UN> constants(const GnArgs& a, const float* mean, const float* rstd, int c) {      // the sample's statistics
+    Consts<V, UN> k;
+#pragma unroll
+    for (int e = 0; e < V; ++e) { k.a[e] = a.gamma ? a.gamma[c + e] : 1.f; k.b[e] = a.beta ? a.beta[c + e] : 0.f; }
+#pragma unroll
+    for (int u = 0; u < V / UN; ++u) { const int g = (c + u * UN) / a.cg; k.mu[u] = mean[g]; k.rs[u] = rstd[g]; }
+#pragma unroll
+    for (int e = 0; e < V; ++e) k.a[e] *= k.rs[e / UN];
+    return k;
+}
+
 // act(z): slope 0 ReLU, (0, 1] LeakyReLU / identity, ACT_SILU z * sigmoid(z)
 template <bool SILU> __device__ __forceinline__ float activate(float z, float slope) {
     if constexpr (SILU) return z * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.44269504f));
     else return z <= 0.f ? (slope == 0.f ? 0.f : slope * z) : z;       // NaN stays NaN
 }
 
-template <int V> struct Consts { float mu[V], a[V], b[V]; };
-template <int V> __device__ __forceinline__ Consts<V> constants(const GnArgs& a, const float* mean, const float* rstd, int c) {      // the sample's statistics
-    Consts<V> k;
+// ------------------------------------------------------------------------------------------------ forward
+// Sums and sums of squares in fp64: the variance is then a difference that loses nothing an fp32 input holds, whatever its mean.
+template <int V, int UN> struct Moments {
+    double s[V / UN], t[V / UN];
+    __device__ __forceinline__ Moments() {
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-        const int g = (c + e) / a.cg;
-        k.mu[e] = mean[g];
-        k.a[e] = rstd[g] * (a.gamma ? a.gamma[c + e] : 1.f);
-        k.b[e] = a.beta ? a.beta[c + e] : 0.f;
+        for (int u = 0; u < V / UN; ++u) s[u] = t[u] = 0.0;
     }
-    return k;
+    __device__ __forceinline__ void add(const float (&f)[V]) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) { const double d = f[e]; s[e / UN] += d; t[e / UN] = fma(d, d, t[e / UN]); }
+    }
+};
+
+template <int DT, int V, int UN>
+__global__ __launch_bounds__(MAX_T) void gn_stats_kernel(const GnArgs a) {
+    extern __shared__ double sh[];
+    const Where w = where<V>(a, blockIdx.x);
+    constexpr int U = 4;
+    Moments<V, UN> m;
+    if (w.on)
+        for (long long v = w.v0 + w.r; v < w.v1; v += U * a.R) {
+            In<DT, V, false> in[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) { in[u].r = {}; if (v + u * a.R < w.v1) in[u].load(a, w.n * a.S + v + u * a.R, w.c); }
+#pragma unroll
+            for (int u = 0; u < U; ++u) { float f[V]; in[u].get(f); m.add(f); }        // (a piece that is not there is zeros)
+        }
+    constexpr int K = V / UN;
+    const int units = a.PT * K;
+    double* s2 = sh + a.R * units;
+    if (w.r < a.R) {
+#pragma unroll
+        for (int u = 0; u < K; ++u) { const int i = w.r * units + (int)(threadIdx.x % a.PT) * K + u; sh[i] = m.s[u]; s2[i] = m.t[u]; }
+    }
+    __syncthreads();
+    const int all = a.C / UN, first = w.tile * units;
+    double* o = a.part + (size_t)(blockIdx.x / a.tiles) * all * 2;
+    sum_rows(sh, s2, a.R, units, [&](int u, double x, double y) { if (first + u < all) { o[(first + u) * 2] = x; o[(first + u) * 2 + 1] = y; } });
 }
 
-template <int DT, int V, bool CK, bool SILU, bool KEEP>
+template <int DT, int V, int UN, bool CK, bool SILU, bool KEEP>
 __global__ __launch_bounds__(MAX_T) void gn_apply_kernel(const GnArgs a) {
     extern __shared__ double sh[];
     const Where w = where<V>(a, blockIdx.x);
@@ -230,8 +233,8 @@ __global__ __launch_bounds__(MAX_T) void gn_apply_kernel(const GnArgs a) {
         __syncthreads();
         mean = st; rstd = st + a.G;
     }
-    Consts<V> k{};
-    if (w.on) k = constants<V>(a, mean, rstd, w.c);
+    Consts<V, UN> k{};
+    if (w.on) k = constants<V, UN>(a, mean, rstd, w.c);
     // (KEEP: every lane goes round together -- the checkpoint's blocks are 8 lanes)
     for (long long vb = w.v0; vb < w.v1; vb += U * a.R) {
         In<DT, V, CK> in[U]; bool ok[U];
@@ -252,42 +255,114 @@ __global__ __launch_bounds__(MAX_T) void gn_apply_kernel(const GnArgs a) {
                 if (ok[u]) store_codes<V>(c, a.q_out, a.qs_out, row * a.C + w.c);
             }
 #pragma unroll
-            for (int e = 0; e < V; ++e) o[e] = activate<SILU>(__builtin_fmaf(f[e] - k.mu[e], k.a[e], k.b[e]), a.slope);
+            for (int e = 0; e < V; ++e) o[e] = activate<SILU>(__builtin_fmaf(f[e] - k.mu[e / UN], k.a[e], k.b[e]), a.slope);
             if (ok[u]) store_f32<DT, V>((T*)a.out + row * a.out_ldc + w.c, o);
         }
     }
 }
 
-// ------------------------------------------------------------------------------------------------ backward
-// dz = dy act'(z).  On which side of 0 a ReLU's z falls is decided as in exact arithmetic: z's rounding error is below 2^-21 of |(x - mean) rstd gamma|, and a z
-// that small is formed again in fp64 (one element in a few hundred thousand).
-template <bool SILU> __device__ __forceinline__ float dz_of(float x, float g, float mu, float rstd, float gamma, float beta, float a, float slope) {
-    const float p = (x - mu) * a, z = p + beta;
-    if constexpr (SILU) {
-        const float sg = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.44269504f));
-        return g * (sg * (1.f + z * (1.f - sg)));
-    } else {
-        bool pos = z > 0.f;
-        if (fabsf(z) < fabsf(p) * 0x1p-21f) pos = ((double)x - (double)mu) * (double)rstd * (double)gamma + (double)beta > 0.0;
-        return pos ? g : (slope == 0.f ? 0.f : slope * g);
+// Small groups: a workgroup takes ONE sample's bundle of whole groups (one group, or the groups of a piece of 8 channels), keeps its pieces in registers from the
+// statistics to the stores, and needs no records and no second launch.  HELD pieces per thread; thread = (voxel r, piece p) as above, PT pieces to a bundle.
+constexpr int HELD = 4;
+template <int DT, int V, int UN, bool SILU, bool KEEP>
+__global__ __launch_bounds__(MAX_T) void gn_fwd_group_kernel(const GnArgs a) {
+    constexpr int K = V / UN;
+    __shared__ double sh[2 * K * MAX_T / 64];
+    __shared__ float st[2 * K];
+    typedef typename Elem<DT>::T T;
+    const int bundles = a.P / a.PT, n = blockIdx.x / bundles, c0 = (blockIdx.x % bundles) * a.PT * V;
+    const int r = threadIdx.x / a.PT, c = c0 + (threadIdx.x % a.PT) * V;
+    const bool on = r < a.R;
+    In<DT, V, false> in[HELD];
+    Moments<V, UN> m;
+#pragma unroll
+    for (int k = 0; k < HELD; ++k) { in[k].r = {}; if (on && r + k * a.R < a.S) in[k].load(a, n * a.S + r + k * a.R, c); }
+#pragma unroll
+    for (int k = 0; k < HELD; ++k) { float f[V]; in[k].get(f); m.add(f); }
+    // wave, then workgroup.  (K > 1: the bundle is one piece, its units are whole groups or quarters of one: merged by the thread that takes the group)
+    const int G = a.PT * V / a.cg > 0 ? a.PT * V / a.cg : 1, per = K / G > 0 ? K / G : 1, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+#pragma unroll
+    for (int u = 0; u < K; ++u) {
+        const double x = wave_sum(m.s[u]), y = wave_sum(m.t[u]);
+        if ((threadIdx.x & 63) == 0) { sh[2 * (wave * K + u)] = x; sh[2 * (wave * K + u) + 1] = y; }
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < G) {
+        double x = 0.0, y = 0.0;
+        for (int i = 0; i < waves; ++i)
+            for (int u = threadIdx.x * per; u < (int)(threadIdx.x + 1) * per; ++u) { x += sh[2 * (i * K + u)]; y += sh[2 * (i * K + u) + 1]; }
+        float mean, rstd;
+        statistics_of(x, y, a.inv_m, a.eps, mean, rstd);
+        st[threadIdx.x] = mean; st[K + threadIdx.x] = rstd;
+        const size_t g = (size_t)n * a.G + c0 / a.cg + threadIdx.x;
+        a.mean_out[g] = mean; a.rstd_out[g] = rstd;
+    }
+    __syncthreads();
+    Consts<V, UN> k0{};
+    if (on) k0 = constants<V, UN>(a, st - c0 / a.cg, st + K - c0 / a.cg, c);
+#pragma unroll
+    for (int k = 0; k < HELD; ++k) {
+        const int v = r + k * a.R;
+        const bool ok = on && v < a.S;
+        float f[V], o[V];
+        in[k].get(f);
+        const size_t row = (size_t)(n * a.S + v);
+        if constexpr (KEEP) {                // (bundles of whole blocks)
+            const Codes<V> q = encode_block<V>(f);
+            if (ok) store_codes<V>(q, a.q_out, a.qs_out, row * a.C + c);
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e) o[e] = activate<SILU>(__builtin_fmaf(f[e] - k0.mu[e / UN], k0.a[e], k0.b[e]), a.slope);
+        if (ok) store_f32<DT, V>((T*)a.out + row * a.out_ldc + c, o);
     }
 }
 
-template <int V> struct ConstsB { float mu[V], rs[V], ga[V], be[V]; };
-template <int V> __device__ __forceinline__ ConstsB<V> constants_b(const GnArgs& a, int n, int c) {
-    ConstsB<V> k;
+// ------------------------------------------------------------------------------------------------ backward
+// dz = dy act'(z) of a piece; t = x - mean.  On which side of 0 a ReLU's z falls is decided as in exact arithmetic: z's rounding error is below 2^-21 of
+// |t a|, which is |beta| up to a factor 2 where z is that small, and a piece with such a z is decided again in fp64 (one in some ten thousand).  That branch
+// is a loop over the elements with its constants from memory: unrolled, hipcc computes their addresses and conversions in front of the voxel loop and keeps 64 to
+// 100 registers with them (reduce pass: 204 registers instead of 92, two waves per SIMD instead of five).
+template <int V, int UN, bool SILU>
+__device__ __forceinline__ void grad_piece(const GnArgs& a, int n, int c, const float (&x)[V], const float (&g)[V], const Consts<V, UN>& k, float border, float (&dz)[V], float (&t)[V]) {
+    float least = 3.4e38f;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-        const int g = n * a.G + (c + e) / a.cg;
-        k.mu[e] = a.mean[g]; k.rs[e] = a.rstd[g];
-        k.ga[e] = a.gamma ? a.gamma[c + e] : 1.f;
-        k.be[e] = a.beta ? a.beta[c + e] : 0.f;
+        t[e] = x[e] - k.mu[e / UN];
+        const float z = __builtin_fmaf(t[e], k.a[e], k.b[e]);
+        if constexpr (SILU) {
+            const float sg = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.44269504f));
+            dz[e] = g[e] * (sg * (1.f + z * (1.f - sg)));
+        } else {
+            least = fminf(least, fabsf(z));
+            dz[e] = z > 0.f ? g[e] : (a.slope == 0.f ? 0.f : a.slope * g[e]);
+        }
     }
-    return k;
+    if constexpr (!SILU) {
+        if (least < border) {
+#pragma unroll 1
+            for (int e = 0; e < V; ++e) {
+                const size_t i = (size_t)n * a.G + (c + e) / a.cg;
+                const double ga = a.gamma ? (double)a.gamma[c + e] : 1.0, be = a.beta ? (double)a.beta[c + e] : 0.0;
+                float xe = x[0], ge = g[0];
+#pragma unroll
+                for (int j = 1; j < V; ++j) { xe = e == j ? x[j] : xe; ge = e == j ? g[j] : ge; }
+                const bool pos = ((double)xe - (double)a.mean[i]) * (double)a.rstd[i] * ga + be > 0.0;
+                const float d = pos ? ge : (a.slope == 0.f ? 0.f : a.slope * ge);
+#pragma unroll
+                for (int j = 0; j < V; ++j) dz[j] = e == j ? d : dz[j];
+            }
+        }
+    }
+}
+template <int V, int UN> __device__ __forceinline__ float border_of(const Consts<V, UN>& k) {
+    float m = 0.f;
+#pragma unroll
+    for (int e = 0; e < V; ++e) m = fmaxf(m, fabsf(k.b[e]));
+    return m * 0x1p-20f;
 }
 
-// Per-thread sums in fp32 over at most a chunk's voxels / R, everything behind them in fp64.
-template <int DT, int V, bool CK, bool SILU>
+// Per-thread sums of dz and dz t (h = t rstd: the factor comes last) in fp32 over at most a chunk's voxels / R, everything behind them in fp64.
+template <int DT, int V, int UN, bool CK, bool SILU>
 __global__ __launch_bounds__(MAX_T) void gn_bwd_reduce_kernel(const GnArgs a) {
     extern __shared__ float shf[];
     const Where w = where<V>(a, blockIdx.x);
@@ -297,28 +372,27 @@ __global__ __launch_bounds__(MAX_T) void gn_bwd_reduce_kernel(const GnArgs a) {
 #pragma unroll
     for (int e = 0; e < V; ++e) s[e] = t[e] = 0.f;
     if (w.on) {
-        const ConstsB<V> k = constants_b<V>(a, w.n, w.c);
+        const Consts<V, UN> k = constants<V, UN>(a, a.mean + (size_t)w.n * a.G, a.rstd + (size_t)w.n * a.G, w.c);
+        const float border = border_of<V, UN>(k);
         for (long long v = w.v0 + w.r; v < w.v1; v += U * a.R) {
-            In<DT, V, CK> in[U]; Raw<DT, V> dy[U]; bool ok[U];
+            In<DT, V, CK> in[U]; Raw<DT, V> dy[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                ok[u] = v + u * a.R < w.v1;
                 in[u].r = {}; dy[u] = {};
                 const long long row = w.n * a.S + v + u * a.R;
-                if (ok[u]) { in[u].load(a, row, w.c); dy[u] = load_raw<DT, V>((const T*)a.dy + (size_t)row * a.dy_ldc + w.c); }
+                if (v + u * a.R < w.v1) { in[u].load(a, row, w.c); dy[u] = load_raw<DT, V>((const T*)a.dy + (size_t)row * a.dy_ldc + w.c); }
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                float f[V], g[V];
-                in[u].get(f); unpack_raw<DT, V>(dy[u], g);
+                float f[V], g[V], dz[V], d[V];
+                in[u].get(f); unpack_raw<DT, V>(dy[u], g);       // (a piece that is not there has dy = 0)
+                grad_piece<V, UN, SILU>(a, w.n, w.c, f, g, k, border, dz, d);
 #pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    const float dz = dz_of<SILU>(f[e], g[e], k.mu[e], k.rs[e], k.ga[e], k.be[e], k.rs[e] * k.ga[e], a.slope);
-                    const float h = (f[e] - k.mu[e]) * k.rs[e];
-                    if (ok[u]) { s[e] += dz; t[e] = __builtin_fmaf(dz, h, t[e]); }
-                }
+                for (int e = 0; e < V; ++e) { s[e] += dz[e]; t[e] = __builtin_fmaf(dz[e], d[e], t[e]); }
             }
         }
+#pragma unroll
+        for (int e = 0; e < V; ++e) t[e] *= k.rs[e / UN];
     }
     const int units = a.PT * V;
     float* t2 = shf + a.R * units;
@@ -384,22 +458,24 @@ __global__ __launch_bounds__(256) void gn_bwd_finalize_kernel(const double* __re
     } else sum_channels(part, N * chunks, C, (i - N * G) * 16, dgamma, dbeta, sh);
 }
 
-template <int DT, int V, bool CK, bool SILU>
+// dx = a dz - rstd m1 - t rstd^2 m2
+template <int DT, int V, int UN, bool CK, bool SILU>
 __global__ __launch_bounds__(MAX_T) void gn_bwd_apply_kernel(const GnArgs a) {
     extern __shared__ double sh[];
-    if (blockIdx.x < a.sum_wgs) { sum_channels(a.cpart, a.N * a.rec_chunks, a.C, blockIdx.x * 16, a.dgamma, a.dbeta, sh); return; }
+    if ((int)blockIdx.x < a.sum_wgs) { sum_channels(a.cpart, a.N * a.rec_chunks, a.C, blockIdx.x * 16, a.dgamma, a.dbeta, sh); return; }
     const Where w = where<V>(a, blockIdx.x - a.sum_wgs);
     constexpr int U = 2;
     typedef typename Elem<DT>::T T;
-    float m1[V], m2[V];
     if (a.rec) merge_records(a.rec + (size_t)w.n * a.rec_chunks * a.rec_units * 2, a.rec_chunks, a.rec_units, a.rec_per, sh);
     if (!w.on) return;
-    const ConstsB<V> k = constants_b<V>(a, w.n, w.c);
+    const Consts<V, UN> k = constants<V, UN>(a, a.mean + (size_t)w.n * a.G, a.rstd + (size_t)w.n * a.G, w.c);
+    const float border = border_of<V, UN>(k);
+    float c1[V / UN], c2[V / UN];
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-        const int g = (w.c + e) / a.cg;
-        if (a.rec) { m1[e] = (float)(sh[2 * g] * a.inv_m); m2[e] = (float)(sh[2 * g + 1] * a.inv_m); }
-        else { m1[e] = a.m1[w.n * a.G + g]; m2[e] = a.m2[w.n * a.G + g]; }
+    for (int u = 0; u < V / UN; ++u) {
+        const int g = (w.c + u * UN) / a.cg;
+        const float m1 = a.rec ? (float)(sh[2 * g] * a.inv_m) : a.m1[(size_t)w.n * a.G + g], m2 = a.rec ? (float)(sh[2 * g + 1] * a.inv_m) : a.m2[(size_t)w.n * a.G + g];
+        c1[u] = k.rs[u] * m1; c2[u] = k.rs[u] * k.rs[u] * m2;
     }
     for (long long v = w.v0 + w.r; v < w.v1; v += U * a.R) {
         In<DT, V, CK> in[U]; Raw<DT, V> dy[U]; bool ok[U];
@@ -412,14 +488,11 @@ __global__ __launch_bounds__(MAX_T) void gn_bwd_apply_kernel(const GnArgs a) {
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            float f[V], g[V], o[V];
+            float f[V], g[V], dz[V], d[V], o[V];
             in[u].get(f); unpack_raw<DT, V>(dy[u], g);
+            grad_piece<V, UN, SILU>(a, w.n, w.c, f, g, k, border, dz, d);
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const float dz = dz_of<SILU>(f[e], g[e], k.mu[e], k.rs[e], k.ga[e], k.be[e], k.rs[e] * k.ga[e], a.slope);
-                const float h = (f[e] - k.mu[e]) * k.rs[e];
-                o[e] = k.rs[e] * (__builtin_fmaf(k.ga[e], dz, -m1[e]) - h * m2[e]);
-            }
+            for (int e = 0; e < V; ++e) o[e] = __builtin_fmaf(k.a[e], dz[e], -__builtin_fmaf(d[e], c2[e / UN], c1[e / UN]));
             if (ok[u]) store_f32<DT, V>((T*)a.out + (size_t)(w.n * a.S + v + u * a.R) * a.out_ldc + w.c, o);
         }
     }
@@ -428,9 +501,17 @@ __global__ __launch_bounds__(MAX_T) void gn_bwd_apply_kernel(const GnArgs a) {
 // ------------------------------------------------------------------------------------------------ host side
 struct Shape { int N; long long S; int C, G; };
 
+#ifndef GN_STATS_WGS
+#define GN_STATS_WGS 512
+#define GN_APPLY_WGS 1024
+#endif
+constexpr int STATS_WGS = GN_STATS_WGS, APPLY_WGS = GN_APPLY_WGS;
+
+void set_shape(GnArgs& a, const Shape& sh) { a.N = sh.N; a.S = sh.S; a.C = sh.C; a.G = sh.G; a.cg = sh.C / sh.G; a.inv_m = 1.0 / ((double)sh.S * a.cg); }
+
 // mapping of a pass; `target`: workgroups that it asks for (at least one per sample and tile)
 template <int V> void map_pass(GnArgs& a, const Shape& sh, int target, int U, bool keep) {
-    a.N = sh.N; a.S = sh.S; a.C = sh.C; a.G = sh.G; a.cg = sh.C / sh.G;
+    set_shape(a, sh);
     a.P = sh.C / V;
     a.tiles = (a.P + MAX_T - 1) / MAX_T;
     a.PT = (a.P + a.tiles - 1) / a.tiles;
@@ -452,25 +533,16 @@ template <int V> void map_pass(GnArgs& a, const Shape& sh, int target, int U, bo
 dim3 grid_of(const GnArgs& a) { return dim3((unsigned)((long long)a.N * a.chunks * a.tiles)); }
 dim3 block_of(const GnArgs& a) { return dim3((unsigned)((a.R * a.PT + 63) / 64 * 64)); }
 
-#ifndef GN_STATS_WGS
-#define GN_STATS_WGS 512
-#define GN_APPLY_WGS 1024
-#endif
-constexpr int STATS_WGS = GN_STATS_WGS, APPLY_WGS = GN_APPLY_WGS;
-
-template <int V> int unit_of(int cg) {
-    int u = V;
-    while (cg % u) u >>= 1;
-    return u;
-}
+// (UN of the kernels: 8, 4 or 1 channels; the statistics' records have C / UN units)
+int unit_of(int V, int cg) { return V == 8 ? (cg % 8 == 0 ? 8 : cg % 4 == 0 ? 4 : 1) : 1; }
 
 template <int V> size_t fwd_part_doubles(const Shape& sh) {
     GnArgs a{}; map_pass<V>(a, sh, STATS_WGS, 4, false);
-    return (size_t)sh.N * a.chunks * (sh.C / unit_of<V>(sh.C / sh.G)) * 2;
+    return (size_t)sh.N * a.chunks * (sh.C / unit_of(V, sh.C / sh.G)) * 2;
 }
 // what lies in the workspace of a backward pass: channel records, then group records (`merge`) or m1 and m2
 struct BwdSpace { size_t channels, behind; bool merge; };
-template <int V> BwdSpace bwd_space(const GnArgs& a, const Shape& sh) {
+BwdSpace bwd_space(const GnArgs& a, const Shape& sh) {
     BwdSpace b;
     b.merge = a.tiles == 1 && sh.C <= 1024 && sh.G <= MERGE_UNITS && (long long)a.chunks * sh.G <= MERGE_MAX;
     b.channels = align_up((size_t)sh.N * a.chunks * sh.C * 2 * sizeof(double), 256);
@@ -480,80 +552,112 @@ template <int V> BwdSpace bwd_space(const GnArgs& a, const Shape& sh) {
 size_t max2(size_t a, size_t b) { return a > b ? a : b; }
 template <int V> size_t space_of(const Shape& sh) {
     GnArgs a{}; map_pass<V>(a, sh, STATS_WGS, 2, false);
-    const BwdSpace b = bwd_space<V>(a, sh);
+    const BwdSpace b = bwd_space(a, sh);
     return max2(fwd_part_doubles<V>(sh) * sizeof(double), b.channels + b.behind);
 }
 size_t workspace_bytes(const Shape& sh) { return max2(space_of<1>(sh), sh.C % 8 == 0 ? space_of<8>(sh) : 0); }
 size_t merge_lds(const GnArgs& a, int units) { return (size_t)2 * (block_of(a).x + units) * sizeof(double); }
 
-template <int DT, int V, bool CK> void launch_apply(GnArgs a, const Shape& sh, hipStream_t s) {
+#define GN_LAUNCH(KERNEL, GRID, BLOCK, LDS, S, A)                                                                                       \
+    do {                                                                                                                                \
+        if ((A).slope == ACT_SILU) { constexpr bool SILU = true; hipLaunchKernelGGL((KERNEL), GRID, BLOCK, LDS, S, A); }                \
+        else { constexpr bool SILU = false; hipLaunchKernelGGL((KERNEL), GRID, BLOCK, LDS, S, A); }                                     \
+    } while (0)
+
+template <int DT, int V, int UN, bool CK> void launch_apply(GnArgs a, const Shape& sh, hipStream_t s) {
     const bool keep = a.q_out != nullptr;
     map_pass<V>(a, sh, APPLY_WGS, 4, keep);
     const size_t lds = a.rec ? merge_lds(a, a.rec_units) : 0;
-    if (a.slope == ACT_SILU) {
-        if constexpr (V == 8 && !CK) if (keep) { hipLaunchKernelGGL((gn_apply_kernel<DT, V, CK, true, true>), grid_of(a), block_of(a), lds, s, a); return; }
-        hipLaunchKernelGGL((gn_apply_kernel<DT, V, CK, true, false>), grid_of(a), block_of(a), lds, s, a);
-    } else {
-        if constexpr (V == 8 && !CK) if (keep) { hipLaunchKernelGGL((gn_apply_kernel<DT, V, CK, false, true>), grid_of(a), block_of(a), lds, s, a); return; }
-        hipLaunchKernelGGL((gn_apply_kernel<DT, V, CK, false, false>), grid_of(a), block_of(a), lds, s, a);
+    if constexpr (V == 8 && !CK) {
+        if (keep) { GN_LAUNCH((gn_apply_kernel<DT, V, UN, CK, SILU, true>), grid_of(a), block_of(a), lds, s, a); return; }
     }
+    GN_LAUNCH((gn_apply_kernel<DT, V, UN, CK, SILU, false>), grid_of(a), block_of(a), lds, s, a);
 }
 
-template <int DT, int V> int forward(GnArgs a, const Shape& sh, float eps, float* mean, float* rstd, void* ws, hipStream_t s) {
+// One workgroup per group where the pieces of a bundle fit its threads' registers
+template <int DT, int V, int UN> bool forward_group(GnArgs a, const Shape& sh, hipStream_t s) {
+#ifdef GN_GROUP_OFF
+    return false;
+#endif
+    set_shape(a, sh);
+    if (V == 8 && a.cg % 8 != 0 && 8 % a.cg != 0) return false;
+    a.P = sh.C / V;
+    a.PT = a.cg > V ? a.cg / V : 1;
+    if (a.PT > MAX_T || sh.S > (long long)HELD * (MAX_T / a.PT)) return false;
+    const bool keep = a.q_out != nullptr;
+    if (keep && !(V == 8 && a.PT % 8 == 0 && ((uintptr_t)a.q_out & 7) == 0)) return false;
+    a.R = MAX_T / a.PT;
+    for (int t = MAX_T / 2; t >= 64; t /= 2)             // no more threads than pieces
+        if (t / a.PT > 0 && sh.S <= t / a.PT) a.R = t / a.PT;
+    const dim3 grid((unsigned)((long long)sh.N * (a.P / a.PT)));
+    if constexpr (V == 8 && UN == 8) {
+        if (keep) { GN_LAUNCH((gn_fwd_group_kernel<DT, V, UN, SILU, true>), grid, block_of(a), 0, s, a); return true; }
+    }
+    GN_LAUNCH((gn_fwd_group_kernel<DT, V, UN, SILU, false>), grid, block_of(a), 0, s, a);
+    return true;
+}
+
+template <int DT, int V, int UN> int forward(GnArgs a, const Shape& sh, void* ws, hipStream_t s) {
+    if (forward_group<DT, V, UN>(a, sh, s)) { E3_CHECK_HIP(hipGetLastError()); return E3_OK; }
     GnArgs st = a;
     map_pass<V>(st, sh, STATS_WGS, 4, false);
-    st.unit = unit_of<V>(st.cg);
     st.part = (double*)ws;
-    const int units = sh.C / st.unit;
-    hipLaunchKernelGGL((gn_stats_kernel<DT, V>), grid_of(st), block_of(st), (size_t)st.R * st.PT * (V / st.unit) * 2 * sizeof(double), s, st);
-    const double inv_m = 1.0 / ((double)sh.S * st.cg);
-    a.mean = mean; a.rstd = rstd;
-    if ((long long)st.chunks * units <= MERGE_MAX && units <= MERGE_UNITS) {
-        a.rec = st.part; a.rec_chunks = st.chunks; a.rec_units = units; a.rec_per = st.cg / st.unit;
-        a.inv_m = inv_m; a.eps = eps; a.mean_out = mean; a.rstd_out = rstd;
-    } else
-        hipLaunchKernelGGL(gn_finalize_kernel, dim3(sh.N * sh.G), dim3(256), 0, s, st.part, st.chunks, units, st.cg / st.unit, inv_m, eps, mean, rstd);
+    const int units = sh.C / UN, per = st.cg / UN;
+    hipLaunchKernelGGL((gn_stats_kernel<DT, V, UN>), grid_of(st), block_of(st), (size_t)st.R * st.PT * (V / UN) * 2 * sizeof(double), s, st);
+    a.mean = a.mean_out; a.rstd = a.rstd_out;
+    if ((long long)st.chunks * units <= MERGE_MAX && units <= MERGE_UNITS) { a.rec = st.part; a.rec_chunks = st.chunks; a.rec_units = units; a.rec_per = per; }
+    else hipLaunchKernelGGL(gn_finalize_kernel, dim3(sh.N * sh.G), dim3(256), 0, s, st.part, st.chunks, units, per, st.inv_m, a.eps, a.mean_out, a.rstd_out);
     // the checkpoint rides in the apply pass where its blocks are whole there; otherwise it is a pass of its own
-    signed char* q = a.q_out; float* qs = a.qs_out;
     GnArgs m{}; map_pass<V>(m, sh, APPLY_WGS, 4, true);
-    const bool fused = q && V == 8 && m.tiles == 1 && m.R * m.PT <= MAX_T && ((unsigned long long)sh.S * sh.C) % CK_BLOCK == 0 && ((uintptr_t)q & 7) == 0;
-    if (q && !fused) { const int rc = launch_checkpoint8_pack(DT, a.x, a.x_ldc, (long long)sh.N * sh.S, sh.C, q, qs, s); if (rc) return rc; }
-    if (!fused) a.q_out = nullptr;
-    launch_apply<DT, V, false>(a, sh, s);
+    const bool fused = a.q_out && V == 8 && m.tiles == 1 && m.R * m.PT <= MAX_T && ((unsigned long long)sh.S * sh.C) % CK_BLOCK == 0 && ((uintptr_t)a.q_out & 7) == 0;
+    if (a.q_out && !fused) {
+        const int rc = launch_checkpoint8_pack(DT, a.x, a.x_ldc, (long long)sh.N * sh.S, sh.C, a.q_out, a.qs_out, s);
+        if (rc) return rc;
+        a.q_out = nullptr;
+    }
+    launch_apply<DT, V, UN, false>(a, sh, s);
     E3_CHECK_HIP(hipGetLastError());
     return E3_OK;
 }
 
-template <int DT, int V, bool CK> int backward(GnArgs a, const Shape& sh, float* dgamma, float* dbeta, void* ws, hipStream_t s) {
+template <int DT, int V, int UN, bool CK> int backward(GnArgs a, const Shape& sh, void* ws, hipStream_t s) {
     GnArgs st = a;
     map_pass<V>(st, sh, STATS_WGS, 2, false);
     st.part = (double*)ws;
-    const BwdSpace space = bwd_space<V>(st, sh);
+    const BwdSpace space = bwd_space(st, sh);
     void* behind = (char*)ws + space.channels;
-    const bool merge = space.merge;
-    if (merge) st.gpart = (double*)behind;
-    const size_t lds = align_up((size_t)st.R * st.PT * V * 2 * sizeof(float), 8) + (merge ? (size_t)sh.C * 2 * sizeof(double) : 0);
-    if (a.slope == ACT_SILU) hipLaunchKernelGGL((gn_bwd_reduce_kernel<DT, V, CK, true>), grid_of(st), block_of(st), lds, s, st);
-    else hipLaunchKernelGGL((gn_bwd_reduce_kernel<DT, V, CK, false>), grid_of(st), block_of(st), lds, s, st);
+    if (space.merge) st.gpart = (double*)behind;
+    const size_t lds = align_up((size_t)st.R * st.PT * V * 2 * sizeof(float), 8) + (space.merge ? (size_t)sh.C * 2 * sizeof(double) : 0);
+    GN_LAUNCH((gn_bwd_reduce_kernel<DT, V, UN, CK, SILU>), grid_of(st), block_of(st), lds, s, st);
     map_pass<V>(a, sh, APPLY_WGS, 2, false);
-    a.inv_m = 1.0 / ((double)sh.S * st.cg);
     size_t alds = 0;
-    const int sums = (dgamma || dbeta) ? (sh.C + 15) / 16 : 0;
-    if (merge) {
+    const int sums = (a.dgamma || a.dbeta) ? (sh.C + 15) / 16 : 0;
+    if (space.merge) {
         a.rec = st.gpart; a.rec_chunks = st.chunks; a.rec_units = sh.G; a.rec_per = 1;
-        a.cpart = st.part; a.dgamma = dgamma; a.dbeta = dbeta; a.sum_wgs = sums;
+        a.cpart = st.part; a.sum_wgs = sums;
         alds = merge_lds(a, sh.G);
     } else {
         float* m1 = (float*)behind;
         float* m2 = m1 + (size_t)sh.N * sh.G;
-        hipLaunchKernelGGL(gn_bwd_finalize_kernel, dim3(sh.N * sh.G + sums), dim3(256), 0, s, st.part, sh.N, st.chunks, sh.C, sh.G, a.gamma, a.inv_m, m1, m2, dgamma, dbeta);
+        hipLaunchKernelGGL(gn_bwd_finalize_kernel, dim3(sh.N * sh.G + sums), dim3(256), 0, s, st.part, sh.N, st.chunks, sh.C, sh.G, a.gamma, a.inv_m, m1, m2, a.dgamma, a.dbeta);
         a.m1 = m1; a.m2 = m2;
     }
     const dim3 grid(grid_of(a).x + a.sum_wgs);
-    if (a.slope == ACT_SILU) hipLaunchKernelGGL((gn_bwd_apply_kernel<DT, V, CK, true>), grid, block_of(a), alds, s, a);
-    else hipLaunchKernelGGL((gn_bwd_apply_kernel<DT, V, CK, false>), grid, block_of(a), alds, s, a);
+    GN_LAUNCH((gn_bwd_apply_kernel<DT, V, UN, CK, SILU>), grid, block_of(a), alds, s, a);
     E3_CHECK_HIP(hipGetLastError());
     return E3_OK;
+}
+
+// f(DT, V, UN) as compile-time constants
+template <int I> using Int = std::integral_constant<int, I>;
+template <int DT, typename F> int by_pieces(bool v8, int cg, F f) {
+    if (!v8) return f(Int<DT>(), Int<1>(), Int<1>());
+    if (cg % 8 == 0) return f(Int<DT>(), Int<8>(), Int<8>());
+    if (cg % 4 == 0) return f(Int<DT>(), Int<8>(), Int<4>());
+    return f(Int<DT>(), Int<8>(), Int<1>());
+}
+template <typename F> int by_type(int dtype, bool v8, int cg, F f) {
+    return dtype == DT_F32 ? by_pieces<DT_F32>(v8, cg, f) : dtype == DT_BF16 ? by_pieces<DT_BF16>(v8, cg, f) : by_pieces<DT_F16>(v8, cg, f);
 }
 
 bool act_ok(float slope) { return (slope >= 0.f && slope <= 1.f) || slope == ACT_SILU; }
@@ -591,16 +695,9 @@ int e3_group_norm_act_fwd(void* stream, int dtype, const void* x, int x_ldc, con
     E3_REQUIRE(workspace_bytes_ >= workspace_bytes(sh), E3_ERR_WORKSPACE, "workspace too small");
     GnArgs a{};
     a.x = x; a.x_ldc = x_ldc; a.out = y; a.out_ldc = y_ldc; a.gamma = gamma; a.beta = beta; a.slope = act_slope; a.q_out = q; a.qs_out = q_scale;
+    a.eps = eps; a.mean_out = mean; a.rstd_out = rstd;
     const bool v8 = rows_by_8(dtype, x, x_ldc, C) && rows_by_8(dtype, y, y_ldc, C);
-    const hipStream_t s = (hipStream_t)stream;
-    switch (dtype * 2 + v8) {
-        case 0: return forward<DT_F32, 1>(a, sh, eps, mean, rstd, workspace, s);
-        case 1: return forward<DT_F32, 8>(a, sh, eps, mean, rstd, workspace, s);
-        case 2: return forward<DT_BF16, 1>(a, sh, eps, mean, rstd, workspace, s);
-        case 3: return forward<DT_BF16, 8>(a, sh, eps, mean, rstd, workspace, s);
-        case 4: return forward<DT_F16, 1>(a, sh, eps, mean, rstd, workspace, s);
-        default: return forward<DT_F16, 8>(a, sh, eps, mean, rstd, workspace, s);
-    }
+    return by_type(dtype, v8, C / G, [&](auto dt, auto v, auto un) { return forward<dt.value, v.value, un.value>(a, sh, workspace, (hipStream_t)stream); });
 }
 
 int e3_group_norm_act_apply(void* stream, int dtype, const void* x, int x_ldc, const signed char* q, const float* q_scale, const float* mean, const float* rstd,
@@ -613,21 +710,11 @@ int e3_group_norm_act_apply(void* stream, int dtype, const void* x, int x_ldc, c
     GnArgs a{};
     a.x = x; a.x_ldc = x_ldc; a.q = q; a.qs = q_scale; a.out = y; a.out_ldc = y_ldc; a.mean = mean; a.rstd = rstd; a.gamma = gamma; a.beta = beta; a.slope = act_slope;
     const bool v8 = (x ? rows_by_8(dtype, x, x_ldc, C) : C % 8 == 0 && ((uintptr_t)q & 7) == 0) && rows_by_8(dtype, y, y_ldc, C);
-    const hipStream_t s = (hipStream_t)stream;
-    switch ((dtype * 2 + v8) * 2 + (x == nullptr)) {
-        case 0: launch_apply<DT_F32, 1, false>(a, sh, s); break;
-        case 1: launch_apply<DT_F32, 1, true>(a, sh, s); break;
-        case 2: launch_apply<DT_F32, 8, false>(a, sh, s); break;
-        case 3: launch_apply<DT_F32, 8, true>(a, sh, s); break;
-        case 4: launch_apply<DT_BF16, 1, false>(a, sh, s); break;
-        case 5: launch_apply<DT_BF16, 1, true>(a, sh, s); break;
-        case 6: launch_apply<DT_BF16, 8, false>(a, sh, s); break;
-        case 7: launch_apply<DT_BF16, 8, true>(a, sh, s); break;
-        case 8: launch_apply<DT_F16, 1, false>(a, sh, s); break;
-        case 9: launch_apply<DT_F16, 1, true>(a, sh, s); break;
-        case 10: launch_apply<DT_F16, 8, false>(a, sh, s); break;
-        default: launch_apply<DT_F16, 8, true>(a, sh, s); break;
-    }
+    by_type(dtype, v8, C / G, [&](auto dt, auto v, auto un) {
+        if (x) launch_apply<dt.value, v.value, un.value, false>(a, sh, (hipStream_t)stream);
+        else launch_apply<dt.value, v.value, un.value, true>(a, sh, (hipStream_t)stream);
+        return E3_OK;
+    });
     E3_CHECK_HIP(hipGetLastError());
     return E3_OK;
 }
@@ -643,23 +730,12 @@ int e3_group_norm_act_bwd(void* stream, int dtype, const void* x, int x_ldc, con
     E3_REQUIRE(workspace_bytes_ >= workspace_bytes(sh), E3_ERR_WORKSPACE, "workspace too small");
     GnArgs a{};
     a.x = x; a.x_ldc = x_ldc; a.q = q; a.qs = q_scale; a.dy = dy; a.dy_ldc = dy_ldc; a.out = dx; a.out_ldc = dx_ldc;
-    a.mean = mean; a.rstd = rstd; a.gamma = gamma; a.beta = beta; a.slope = act_slope;
+    a.mean = mean; a.rstd = rstd; a.gamma = gamma; a.beta = beta; a.slope = act_slope; a.dgamma = dgamma; a.dbeta = dbeta;
     const bool v8 = (x ? rows_by_8(dtype, x, x_ldc, C) : C % 8 == 0 && ((uintptr_t)q & 7) == 0) && rows_by_8(dtype, dy, dy_ldc, C) && rows_by_8(dtype, dx, dx_ldc, C);
-    const hipStream_t s = (hipStream_t)stream;
-    switch ((dtype * 2 + v8) * 2 + (x == nullptr)) {
-        case 0: return backward<DT_F32, 1, false>(a, sh, dgamma, dbeta, workspace, s);
-        case 1: return backward<DT_F32, 1, true>(a, sh, dgamma, dbeta, workspace, s);
-        case 2: return backward<DT_F32, 8, false>(a, sh, dgamma, dbeta, workspace, s);
-        case 3: return backward<DT_F32, 8, true>(a, sh, dgamma, dbeta, workspace, s);
-        case 4: return backward<DT_BF16, 1, false>(a, sh, dgamma, dbeta, workspace, s);
-        case 5: return backward<DT_BF16, 1, true>(a, sh, dgamma, dbeta, workspace, s);
-        case 6: return backward<DT_BF16, 8, false>(a, sh, dgamma, dbeta, workspace, s);
-        case 7: return backward<DT_BF16, 8, true>(a, sh, dgamma, dbeta, workspace, s);
-        case 8: return backward<DT_F16, 1, false>(a, sh, dgamma, dbeta, workspace, s);
-        case 9: return backward<DT_F16, 1, true>(a, sh, dgamma, dbeta, workspace, s);
-        case 10: return backward<DT_F16, 8, false>(a, sh, dgamma, dbeta, workspace, s);
-        default: return backward<DT_F16, 8, true>(a, sh, dgamma, dbeta, workspace, s);
-    }
+    return by_type(dtype, v8, C / G, [&](auto dt, auto v, auto un) {
+        return x ? backward<dt.value, v.value, un.value, false>(a, sh, workspace, (hipStream_t)stream)
+                 : backward<dt.value, v.value, un.value, true>(a, sh, workspace, (hipStream_t)stream);
+    });
 }
 
 }  // extern "C"
