@@ -31,16 +31,18 @@ template <int DT> __device__ __forceinline__ typename Elem<DT>::T from_f32(float
     else return __builtin_bit_cast(unsigned short, (_Float16)f);
 }
 
-// V consecutive channels of a voxel as they lie in memory: V = 8 with 16-byte accesses (C, row length and address in multiples of 8 elements / 16 bytes), or V = 1
+// V consecutive channels of a voxel as they lie in memory: a piece of 16 bytes (V = wide_of(type): 4 fp32, 8 16-bit elements; C, row length and address in
+// multiples of it), or V = 1.  (8 fp32 elements per lane, two accesses that each fill half of every line: the pass that restores a checkpoint 89 us instead of
+// 62 for 268 MB of output.)
 template <int DT, int V> struct Raw { typename Elem<DT>::T v; };
-template <> struct Raw<DT_F32, 8> { f32x4 lo, hi; };
+template <> struct Raw<DT_F32, 4> { f32x4 v; };
 template <> struct Raw<DT_BF16, 8> { u16x8 v; };
 template <> struct Raw<DT_F16, 8> { u16x8 v; };
 
 template <int DT, int V> __device__ __forceinline__ Raw<DT, V> load_raw(const typename Elem<DT>::T* p) {
     Raw<DT, V> r;
     if constexpr (V == 1) r.v = *p;
-    else if constexpr (DT == DT_F32) { r.lo = *reinterpret_cast<const f32x4*>(p); r.hi = *reinterpret_cast<const f32x4*>(p + 4); }
+    else if constexpr (DT == DT_F32) r.v = *reinterpret_cast<const f32x4*>(p);
     else r.v = *reinterpret_cast<const u16x8*>(p);
     return r;
 }
@@ -48,7 +50,7 @@ template <int DT, int V> __device__ __forceinline__ void unpack_raw(const Raw<DT
     if constexpr (V == 1) f[0] = to_f32<DT>(r.v);
     else if constexpr (DT == DT_F32) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) { f[e] = r.lo[e]; f[e + 4] = r.hi[e]; }
+        for (int e = 0; e < 4; ++e) f[e] = r.v[e];
     } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) f[e] = to_f32<DT>(r.v[e]);
@@ -58,7 +60,6 @@ template <int DT, int V> __device__ __forceinline__ void store_f32(typename Elem
     if constexpr (V == 1) *p = from_f32<DT>(f[0]);
     else if constexpr (DT == DT_F32) {
         *reinterpret_cast<f32x4*>(p) = f32x4{f[0], f[1], f[2], f[3]};
-        *reinterpret_cast<f32x4*>(p + 4) = f32x4{f[4], f[5], f[6], f[7]};
     } else {
         u16x8 o;
 #pragma unroll
@@ -68,11 +69,14 @@ template <int DT, int V> __device__ __forceinline__ void store_f32(typename Elem
 }
 
 // V codes of a checkpoint and their scale
-template <int V> struct RawQ { uint2 q; float s; };
-template <> struct RawQ<1> { signed char q; float s; };
+template <int V> struct RawQ { signed char q; float s; };
+template <> struct RawQ<4> { unsigned q[1]; float s; };
+template <> struct RawQ<8> { unsigned q[2]; float s; };
 template <int V> __device__ __forceinline__ RawQ<V> load_q(const signed char* q, const float* scale, size_t e) {       // e: flat element, a multiple of V
     RawQ<V> r;
-    if constexpr (V == 1) r.q = q[e]; else r.q = *reinterpret_cast<const uint2*>(q + e);
+    if constexpr (V == 1) r.q = q[e];
+    else if constexpr (V == 4) r.q[0] = *reinterpret_cast<const unsigned*>(q + e);
+    else { const uint2 t = *reinterpret_cast<const uint2*>(q + e); r.q[0] = t.x; r.q[1] = t.y; }
     r.s = scale[e / CK_BLOCK];
     return r;
 }
@@ -81,11 +85,19 @@ template <int V> __device__ __forceinline__ void unpack_q(const RawQ<V>& r, floa
     if constexpr (V == 1) f[0] = (float)r.q * r.s;
     else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            f[e] = (float)(signed char)(r.q.x >> (8 * e)) * r.s;
-            f[e + 4] = (float)(signed char)(r.q.y >> (8 * e)) * r.s;
-        }
+        for (int e = 0; e < V; ++e) f[e] = (float)(signed char)(r.q[e / 4] >> (8 * (e % 4))) * r.s;
     }
+}
+
+// maximum over groups of 2^k consecutive lanes: inside a row of 16 lanes with DPP (neighbour, pair, half row, row; each step's partner holds the other half's
+// maximum), beyond with permutes
+template <int LANES> __device__ __forceinline__ unsigned group_max(unsigned m) {
+    m = max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xf, 0xf, false));               // quad_perm 1 0 3 2
+    m = max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xf, 0xf, false));               // quad_perm 2 3 0 1
+    m = max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x141, 0xf, 0xf, false));              // row_half_mirror
+    if constexpr (LANES >= 16) m = max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x140, 0xf, 0xf, false));      // row_mirror
+    if constexpr (LANES == 64) { m = max(m, (unsigned)__shfl_xor((int)m, 16)); m = max(m, (unsigned)__shfl_xor((int)m, 32)); }
+    return m;
 }
 
 // A block's scale and codes from the values of its lanes: 64 / V consecutive lanes of a wave hold one block, V consecutive elements each (lanes outside the tensor
@@ -95,8 +107,7 @@ template <int V> __device__ __forceinline__ Codes<V> encode_block(const float (&
     unsigned m = 0;
 #pragma unroll
     for (int e = 0; e < V; ++e) m = max(m, __float_as_uint(f[e]) & 0x7fffffffu);
-#pragma unroll
-    for (int o = 1; o < CK_BLOCK / V; o <<= 1) m = max(m, (unsigned)__shfl_xor((int)m, o));
+    m = group_max<CK_BLOCK / V>(m);
     const float amax = __uint_as_float(m);
     const bool none = m < __float_as_uint(CK_TINY), bad = m >= 0x7f800000u;
     const float inv = (none || bad) ? 0.f : 127.f / amax;
@@ -109,19 +120,20 @@ template <int V> __device__ __forceinline__ Codes<V> encode_block(const float (&
 template <int V> __device__ __forceinline__ void store_codes(const Codes<V>& c, signed char* q, float* scale, size_t e) {
     if constexpr (V == 1) q[e] = c.q[0];
     else {
-        unsigned lo = 0, hi = 0;
+        unsigned w[V / 4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) { lo |= (unsigned)(unsigned char)c.q[k] << (8 * k); hi |= (unsigned)(unsigned char)c.q[k + 4] << (8 * k); }
-        *reinterpret_cast<uint2*>(q + e) = make_uint2(lo, hi);
+        for (int k = 0; k < V; ++k) { const unsigned b = (unsigned)(unsigned char)c.q[k] << (8 * (k % 4)); w[k / 4] = k % 4 ? w[k / 4] | b : b; }
+        if constexpr (V == 4) *reinterpret_cast<unsigned*>(q + e) = w[0];
+        else *reinterpret_cast<uint2*>(q + e) = make_uint2(w[0], w[V / 4 - 1]);
     }
     if (e % CK_BLOCK == 0) scale[e / CK_BLOCK] = c.scale;
 }
 
 inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
-// whether the rows of a view allow 16-byte pieces of 8 channels
-inline bool rows_by_8(int dt, const void* p, int ldc, int C) {
-    return C % 8 == 0 && aligned16(p) && ldc % (dt == DT_F32 ? 4 : 8) == 0;
-}
+constexpr int wide_of(int dt) { return dt == DT_F32 ? 4 : 8; }
+// whether the rows of a view, or the codes of a checkpoint, allow 16-byte pieces
+inline bool wide_rows(int dt, const void* p, int ldc, int C) { return C % wide_of(dt) == 0 && aligned16(p) && ldc % wide_of(dt) == 0; }
+inline bool wide_codes(int dt, const void* q, int C) { return C % wide_of(dt) == 0 && (uintptr_t)q % wide_of(dt) == 0; }
 
 }  // namespace e3n
 

@@ -23,7 +23,7 @@ template <int V, bool DENSE> __device__ __forceinline__ size_t piece_offset(size
 template <int DT, int V, bool DENSE>
 __global__ __launch_bounds__(BT) void checkpoint8_pack_kernel(const typename Elem<DT>::T* __restrict__ x, int ldc, int C, size_t n,
                                                               signed char* __restrict__ q, float* __restrict__ scale) {
-    constexpr int U = 4;                                     // pieces in flight per lane
+    constexpr int U = DT == DT_F32 ? 8 : 4;                  // pieces in flight per lane
     const size_t step = (size_t)gridDim.x * BT * V;
     // (the loop's condition is the workgroup's: every lane of a wave reaches the reduction inside encode_block)
     for (size_t b0 = (size_t)blockIdx.x * BT * V; b0 < n; b0 += U * step) {
@@ -48,7 +48,7 @@ __global__ __launch_bounds__(BT) void checkpoint8_pack_kernel(const typename Ele
 template <int DT, int V, bool DENSE>
 __global__ __launch_bounds__(BT) void checkpoint8_unpack_kernel(const signed char* __restrict__ q, const float* __restrict__ scale, size_t n, int C, int ldc,
                                                                 typename Elem<DT>::T* __restrict__ y) {
-    constexpr int U = 4;
+    constexpr int U = DT == DT_F32 ? 8 : 4;
     const size_t step = (size_t)gridDim.x * BT * V;
     for (size_t e0 = ((size_t)blockIdx.x * BT + threadIdx.x) * V; e0 < n; e0 += U * step) {
         RawQ<V> raw[U];
@@ -81,9 +81,9 @@ void unpack_typed(const signed char* q, const float* scale, size_t n, int C, voi
     else hipLaunchKernelGGL((checkpoint8_unpack_kernel<DT, V, false>), dim3(grid_for(n, V)), dim3(BT), 0, s, q, scale, n, C, ldc, (P)y);
 }
 
-// a flat tensor of rows without gaps is cut at multiples of 8 whatever its channel count
-bool by_8(int dt, const void* p, int ldc, int C, size_t n, const void* q) {
-    return ((uintptr_t)q & 7) == 0 && (ldc == C ? n % 8 == 0 && aligned16(p) : rows_by_8(dt, p, ldc, C));
+// a flat tensor of rows without gaps is cut into pieces whatever its channel count
+bool wide(int dt, const void* p, int ldc, int C, size_t n, const void* q) {
+    return (uintptr_t)q % wide_of(dt) == 0 && (ldc == C ? n % wide_of(dt) == 0 && aligned16(p) : wide_rows(dt, p, ldc, C));
 }
 
 }  // namespace
@@ -91,10 +91,9 @@ bool by_8(int dt, const void* p, int ldc, int C, size_t n, const void* q) {
 int launch_checkpoint8_pack(int dt, const void* x, int x_ldc, long long vox, int C, signed char* q, float* scale, hipStream_t s) {
     const size_t n = (size_t)vox * C;
     if (n == 0) return E3_OK;
-    const bool v8 = by_8(dt, x, x_ldc, C, n, q);
-    switch (dt * 2 + v8) {
+    switch (dt * 2 + wide(dt, x, x_ldc, C, n, q)) {
         case 0: pack_typed<DT_F32, 1>(x, x_ldc, n, C, q, scale, s); break;
-        case 1: pack_typed<DT_F32, 8>(x, x_ldc, n, C, q, scale, s); break;
+        case 1: pack_typed<DT_F32, 4>(x, x_ldc, n, C, q, scale, s); break;
         case 2: pack_typed<DT_BF16, 1>(x, x_ldc, n, C, q, scale, s); break;
         case 3: pack_typed<DT_BF16, 8>(x, x_ldc, n, C, q, scale, s); break;
         case 4: pack_typed<DT_F16, 1>(x, x_ldc, n, C, q, scale, s); break;
@@ -107,10 +106,9 @@ int launch_checkpoint8_pack(int dt, const void* x, int x_ldc, long long vox, int
 int launch_checkpoint8_unpack(int dt, const signed char* q, const float* scale, long long vox, int C, void* y, int y_ldc, hipStream_t s) {
     const size_t n = (size_t)vox * C;
     if (n == 0) return E3_OK;
-    const bool v8 = by_8(dt, y, y_ldc, C, n, q);
-    switch (dt * 2 + v8) {
+    switch (dt * 2 + wide(dt, y, y_ldc, C, n, q)) {
         case 0: unpack_typed<DT_F32, 1>(q, scale, n, C, y, y_ldc, s); break;
-        case 1: unpack_typed<DT_F32, 8>(q, scale, n, C, y, y_ldc, s); break;
+        case 1: unpack_typed<DT_F32, 4>(q, scale, n, C, y, y_ldc, s); break;
         case 2: unpack_typed<DT_BF16, 1>(q, scale, n, C, y, y_ldc, s); break;
         case 3: unpack_typed<DT_BF16, 8>(q, scale, n, C, y, y_ldc, s); break;
         case 4: unpack_typed<DT_F16, 1>(q, scale, n, C, y, y_ldc, s); break;

@@ -5,7 +5,7 @@
 //     dz = dy act'(z),  h = (x - mean) rstd,  dgamma = sum dz h,  dbeta = sum dz  (over samples and voxels)
 //     dx = rstd (gamma dz - m1 - h m2),  m1 = mean over the group of gamma dz,  m2 = of gamma dz h
 //
-// All kernels are streaming passes with one mapping: a thread keeps V consecutive channels (V = 8: 16-byte accesses; V = 1 for rows that do not allow them) and
+// All kernels are streaming passes with one mapping: a thread keeps V consecutive channels (16 bytes: 4 fp32, 8 16-bit elements; V = 1 for rows that do not allow it) and
 // walks the voxels of its workgroup's chunk, so that the per-channel constants stay in registers; consecutive threads take consecutive pieces of a voxel, then
 // consecutive voxels.  A workgroup works on one chunk of one sample and, for more than 512 pieces per voxel, on one tile of its channels.  UN is the number of
 // consecutive channels of a piece that surely share a group (8, 4 or 1): V / UN constants or sums per thread instead of V, which decides the register count.
@@ -25,6 +25,9 @@ using namespace e3n;
 namespace {
 
 constexpr int MAX_T = 512;                   // threads of a workgroup, at most
+// pieces that a thread has in flight: a pass that reads one tensor, one that reads two
+template <int V> constexpr int U1 = V == 8 ? 4 : 8;
+template <int V> constexpr int U2 = V == 8 ? 2 : 4;
 
 struct GnArgs {
     const void* x; int x_ldc;                // the input, or (x == nullptr) its checkpoint
@@ -193,7 +196,7 @@ template <int DT, int V, int UN>
 __global__ __launch_bounds__(MAX_T) void gn_stats_kernel(const GnArgs a) {
     extern __shared__ double sh[];
     const Where w = where<V>(a, blockIdx.x);
-    constexpr int U = 4;
+    constexpr int U = U1<V>;
     Moments<V, UN> m;
     if (w.on)
         for (long long v = w.v0 + w.r; v < w.v1; v += U * a.R) {
@@ -220,8 +223,22 @@ template <int DT, int V, int UN, bool CK, bool SILU, bool KEEP>
 __global__ __launch_bounds__(MAX_T) void gn_apply_kernel(const GnArgs a) {
     extern __shared__ double sh[];
     const Where w = where<V>(a, blockIdx.x);
-    constexpr int U = 4;
+    constexpr int U = U1<V>;
     typedef typename Elem<DT>::T T;
+    In<DT, V, CK> in[U]; bool ok[U];
+    auto load = [&](long long vb) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const long long v = vb + w.r + u * a.R;
+            ok[u] = w.on && v < w.v1;
+            in[u].r = {};
+            if (ok[u]) in[u].load(a, w.n * a.S + v, w.c);
+        }
+    };
+    // from the chunk's end to its start: what the statistics pass read last is still in the memory-side cache.  The first step is requested in front of the merge
+    const int step = U * a.R;
+    long long vb = w.v0 + (w.v1 - w.v0 - 1) / step * step;
+    load(vb);
     const float* mean = a.mean + (size_t)w.n * a.G; const float* rstd = a.rstd + (size_t)w.n * a.G;
     if (a.rec) {                             // (uniform)
         merge_records(a.rec + (size_t)w.n * a.rec_chunks * a.rec_units * 2, a.rec_chunks, a.rec_units, a.rec_per, sh);
@@ -236,15 +253,7 @@ __global__ __launch_bounds__(MAX_T) void gn_apply_kernel(const GnArgs a) {
     Consts<V, UN> k{};
     if (w.on) k = constants<V, UN>(a, mean, rstd, w.c);
     // (KEEP: every lane goes round together -- the checkpoint's blocks are 8 lanes)
-    for (long long vb = w.v0; vb < w.v1; vb += U * a.R) {
-        In<DT, V, CK> in[U]; bool ok[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const long long v = vb + w.r + u * a.R;
-            ok[u] = w.on && v < w.v1;
-            in[u].r = {};
-            if (ok[u]) in[u].load(a, w.n * a.S + v, w.c);
-        }
+    for (;;) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             float f[V], o[V];
@@ -258,12 +267,15 @@ __global__ __launch_bounds__(MAX_T) void gn_apply_kernel(const GnArgs a) {
             for (int e = 0; e < V; ++e) o[e] = activate<SILU>(__builtin_fmaf(f[e] - k.mu[e / UN], k.a[e], k.b[e]), a.slope);
             if (ok[u]) store_f32<DT, V>((T*)a.out + row * a.out_ldc + w.c, o);
         }
+        vb -= step;
+        if (vb < w.v0) break;
+        load(vb);
     }
 }
 
-// Small groups: a workgroup takes ONE sample's bundle of whole groups (one group, or the groups of a piece of 8 channels), keeps its pieces in registers from the
-// statistics to the stores, and needs no records and no second launch.  HELD pieces per thread; thread = (voxel r, piece p) as above, PT pieces to a bundle.
-constexpr int HELD = 4;
+// Small groups: a workgroup takes ONE sample's bundle of whole groups (one group, or the groups of a piece), keeps its pieces in registers from the
+// statistics to the stores, and needs no records and no second launch.  HELD<V> pieces per thread; thread = (voxel r, piece p) as above, PT pieces to a bundle.
+template <int V> constexpr int HELD = U1<V>;
 template <int DT, int V, int UN, bool SILU, bool KEEP>
 __global__ __launch_bounds__(MAX_T) void gn_fwd_group_kernel(const GnArgs a) {
     constexpr int K = V / UN;
@@ -273,12 +285,12 @@ __global__ __launch_bounds__(MAX_T) void gn_fwd_group_kernel(const GnArgs a) {
     const int bundles = a.P / a.PT, n = blockIdx.x / bundles, c0 = (blockIdx.x % bundles) * a.PT * V;
     const int r = threadIdx.x / a.PT, c = c0 + (threadIdx.x % a.PT) * V;
     const bool on = r < a.R;
-    In<DT, V, false> in[HELD];
+    In<DT, V, false> in[HELD<V>];
     Moments<V, UN> m;
 #pragma unroll
-    for (int k = 0; k < HELD; ++k) { in[k].r = {}; if (on && r + k * a.R < a.S) in[k].load(a, n * a.S + r + k * a.R, c); }
+    for (int k = 0; k < HELD<V>; ++k) { in[k].r = {}; if (on && r + k * a.R < a.S) in[k].load(a, n * a.S + r + k * a.R, c); }
 #pragma unroll
-    for (int k = 0; k < HELD; ++k) { float f[V]; in[k].get(f); m.add(f); }
+    for (int k = 0; k < HELD<V>; ++k) { float f[V]; in[k].get(f); m.add(f); }
     // wave, then workgroup.  (K > 1: the bundle is one piece, its units are whole groups or quarters of one: merged by the thread that takes the group)
     const int G = a.PT * V / a.cg > 0 ? a.PT * V / a.cg : 1, per = K / G > 0 ? K / G : 1, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
 #pragma unroll
@@ -301,7 +313,7 @@ __global__ __launch_bounds__(MAX_T) void gn_fwd_group_kernel(const GnArgs a) {
     Consts<V, UN> k0{};
     if (on) k0 = constants<V, UN>(a, st - c0 / a.cg, st + K - c0 / a.cg, c);
 #pragma unroll
-    for (int k = 0; k < HELD; ++k) {
+    for (int k = 0; k < HELD<V>; ++k) {
         const int v = r + k * a.R;
         const bool ok = on && v < a.S;
         float f[V], o[V];
@@ -366,7 +378,7 @@ template <int DT, int V, int UN, bool CK, bool SILU>
 __global__ __launch_bounds__(MAX_T) void gn_bwd_reduce_kernel(const GnArgs a) {
     extern __shared__ float shf[];
     const Where w = where<V>(a, blockIdx.x);
-    constexpr int U = 2;
+    constexpr int U = U2<V>;
     typedef typename Elem<DT>::T T;
     float s[V], t[V];
 #pragma unroll
@@ -464,8 +476,21 @@ __global__ __launch_bounds__(MAX_T) void gn_bwd_apply_kernel(const GnArgs a) {
     extern __shared__ double sh[];
     if ((int)blockIdx.x < a.sum_wgs) { sum_channels(a.cpart, a.N * a.rec_chunks, a.C, blockIdx.x * 16, a.dgamma, a.dbeta, sh); return; }
     const Where w = where<V>(a, blockIdx.x - a.sum_wgs);
-    constexpr int U = 2;
+    constexpr int U = U2<V>;
     typedef typename Elem<DT>::T T;
+    In<DT, V, CK> in[U]; Raw<DT, V> dy[U]; bool ok[U];
+    auto load = [&](long long vb) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const long long v = vb + w.r + u * a.R, row = w.n * a.S + v;
+            ok[u] = w.on && v < w.v1;
+            in[u].r = {}; dy[u] = {};
+            if (ok[u]) { in[u].load(a, row, w.c); dy[u] = load_raw<DT, V>((const T*)a.dy + (size_t)row * a.dy_ldc + w.c); }
+        }
+    };
+    const int step = U * a.R;                // (from the end, as in the forward)
+    long long vb = w.v0 + (w.v1 - w.v0 - 1) / step * step;
+    load(vb);
     if (a.rec) merge_records(a.rec + (size_t)w.n * a.rec_chunks * a.rec_units * 2, a.rec_chunks, a.rec_units, a.rec_per, sh);
     if (!w.on) return;
     const Consts<V, UN> k = constants<V, UN>(a, a.mean + (size_t)w.n * a.G, a.rstd + (size_t)w.n * a.G, w.c);
@@ -477,15 +502,7 @@ __global__ __launch_bounds__(MAX_T) void gn_bwd_apply_kernel(const GnArgs a) {
         const float m1 = a.rec ? (float)(sh[2 * g] * a.inv_m) : a.m1[(size_t)w.n * a.G + g], m2 = a.rec ? (float)(sh[2 * g + 1] * a.inv_m) : a.m2[(size_t)w.n * a.G + g];
         c1[u] = k.rs[u] * m1; c2[u] = k.rs[u] * k.rs[u] * m2;
     }
-    for (long long v = w.v0 + w.r; v < w.v1; v += U * a.R) {
-        In<DT, V, CK> in[U]; Raw<DT, V> dy[U]; bool ok[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            ok[u] = v + u * a.R < w.v1;
-            in[u].r = {}; dy[u] = {};
-            const long long row = w.n * a.S + v + u * a.R;
-            if (ok[u]) { in[u].load(a, row, w.c); dy[u] = load_raw<DT, V>((const T*)a.dy + (size_t)row * a.dy_ldc + w.c); }
-        }
+    for (;;) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             float f[V], g[V], dz[V], d[V], o[V];
@@ -493,8 +510,11 @@ __global__ __launch_bounds__(MAX_T) void gn_bwd_apply_kernel(const GnArgs a) {
             grad_piece<V, UN, SILU>(a, w.n, w.c, f, g, k, border, dz, d);
 #pragma unroll
             for (int e = 0; e < V; ++e) o[e] = __builtin_fmaf(k.a[e], dz[e], -__builtin_fmaf(d[e], c2[e / UN], c1[e / UN]));
-            if (ok[u]) store_f32<DT, V>((T*)a.out + (size_t)(w.n * a.S + v + u * a.R) * a.out_ldc + w.c, o);
+            if (ok[u]) store_f32<DT, V>((T*)a.out + (size_t)(w.n * a.S + vb + w.r + u * a.R) * a.out_ldc + w.c, o);
         }
+        vb -= step;
+        if (vb < w.v0) break;
+        load(vb);
     }
 }
 
@@ -503,7 +523,8 @@ struct Shape { int N; long long S; int C, G; };
 
 #ifndef GN_STATS_WGS
 #define GN_STATS_WGS 512
-#define GN_APPLY_WGS 1024
+#define GN_APPLY_WGS 512
+#define GN_BT 256
 #endif
 constexpr int STATS_WGS = GN_STATS_WGS, APPLY_WGS = GN_APPLY_WGS;
 
@@ -515,9 +536,9 @@ template <int V> void map_pass(GnArgs& a, const Shape& sh, int target, int U, bo
     a.P = sh.C / V;
     a.tiles = (a.P + MAX_T - 1) / MAX_T;
     a.PT = (a.P + a.tiles - 1) / a.tiles;
-    a.R = 256 / a.PT > 0 ? 256 / a.PT : 1;
+    a.R = GN_BT / a.PT > 0 ? GN_BT / a.PT : 1;
     if (keep) {                              // whole blocks of 64 elements per workgroup step
-        int k = 8;
+        int k = CK_BLOCK / V;
         for (int p = a.PT; k > 1 && p % 2 == 0; p /= 2) k /= 2;
         a.R = (a.R + k - 1) / k * k;
     }
@@ -533,11 +554,11 @@ template <int V> void map_pass(GnArgs& a, const Shape& sh, int target, int U, bo
 dim3 grid_of(const GnArgs& a) { return dim3((unsigned)((long long)a.N * a.chunks * a.tiles)); }
 dim3 block_of(const GnArgs& a) { return dim3((unsigned)((a.R * a.PT + 63) / 64 * 64)); }
 
-// (UN of the kernels: 8, 4 or 1 channels; the statistics' records have C / UN units)
-int unit_of(int V, int cg) { return V == 8 ? (cg % 8 == 0 ? 8 : cg % 4 == 0 ? 4 : 1) : 1; }
+// (UN of the kernels: the statistics' records have C / UN units)
+int unit_of(int V, int cg) { return V >= 8 && cg % 8 == 0 ? 8 : V >= 4 && cg % 4 == 0 ? 4 : 1; }
 
 template <int V> size_t fwd_part_doubles(const Shape& sh) {
-    GnArgs a{}; map_pass<V>(a, sh, STATS_WGS, 4, false);
+    GnArgs a{}; map_pass<V>(a, sh, STATS_WGS, U1<V>, false);
     return (size_t)sh.N * a.chunks * (sh.C / unit_of(V, sh.C / sh.G)) * 2;
 }
 // what lies in the workspace of a backward pass: channel records, then group records (`merge`) or m1 and m2
@@ -551,11 +572,13 @@ BwdSpace bwd_space(const GnArgs& a, const Shape& sh) {
 }
 size_t max2(size_t a, size_t b) { return a > b ? a : b; }
 template <int V> size_t space_of(const Shape& sh) {
-    GnArgs a{}; map_pass<V>(a, sh, STATS_WGS, 2, false);
+    GnArgs a{}; map_pass<V>(a, sh, STATS_WGS, U2<V>, false);
     const BwdSpace b = bwd_space(a, sh);
     return max2(fwd_part_doubles<V>(sh) * sizeof(double), b.channels + b.behind);
 }
-size_t workspace_bytes(const Shape& sh) { return max2(space_of<1>(sh), sh.C % 8 == 0 ? space_of<8>(sh) : 0); }
+size_t workspace_bytes(const Shape& sh) {      // (for every type and alignment)
+    return max2(space_of<1>(sh), max2(sh.C % 4 == 0 ? space_of<4>(sh) : 0, sh.C % 8 == 0 ? space_of<8>(sh) : 0));
+}
 size_t merge_lds(const GnArgs& a, int units) { return (size_t)2 * (block_of(a).x + units) * sizeof(double); }
 
 #define GN_LAUNCH(KERNEL, GRID, BLOCK, LDS, S, A)                                                                                       \
@@ -566,9 +589,9 @@ size_t merge_lds(const GnArgs& a, int units) { return (size_t)2 * (block_of(a).x
 
 template <int DT, int V, int UN, bool CK> void launch_apply(GnArgs a, const Shape& sh, hipStream_t s) {
     const bool keep = a.q_out != nullptr;
-    map_pass<V>(a, sh, APPLY_WGS, 4, keep);
+    map_pass<V>(a, sh, APPLY_WGS, U1<V>, keep);
     const size_t lds = a.rec ? merge_lds(a, a.rec_units) : 0;
-    if constexpr (V == 8 && !CK) {
+    if constexpr (V > 1 && !CK) {
         if (keep) { GN_LAUNCH((gn_apply_kernel<DT, V, UN, CK, SILU, true>), grid_of(a), block_of(a), lds, s, a); return; }
     }
     GN_LAUNCH((gn_apply_kernel<DT, V, UN, CK, SILU, false>), grid_of(a), block_of(a), lds, s, a);
@@ -580,17 +603,17 @@ template <int DT, int V, int UN> bool forward_group(GnArgs a, const Shape& sh, h
     return false;
 #endif
     set_shape(a, sh);
-    if (V == 8 && a.cg % 8 != 0 && 8 % a.cg != 0) return false;
+    if (a.cg % V != 0 && V % a.cg != 0) return false;
     a.P = sh.C / V;
     a.PT = a.cg > V ? a.cg / V : 1;
-    if (a.PT > MAX_T || sh.S > (long long)HELD * (MAX_T / a.PT)) return false;
+    if (a.PT > MAX_T || sh.S > (long long)HELD<V> * (MAX_T / a.PT)) return false;
     const bool keep = a.q_out != nullptr;
-    if (keep && !(V == 8 && a.PT % 8 == 0 && ((uintptr_t)a.q_out & 7) == 0)) return false;
+    if (keep && !(V > 1 && a.PT * V % CK_BLOCK == 0 && (uintptr_t)a.q_out % V == 0)) return false;
     a.R = MAX_T / a.PT;
     for (int t = MAX_T / 2; t >= 64; t /= 2)             // no more threads than pieces
         if (t / a.PT > 0 && sh.S <= t / a.PT) a.R = t / a.PT;
     const dim3 grid((unsigned)((long long)sh.N * (a.P / a.PT)));
-    if constexpr (V == 8 && UN == 8) {
+    if constexpr (V > 1 && UN == V) {
         if (keep) { GN_LAUNCH((gn_fwd_group_kernel<DT, V, UN, SILU, true>), grid, block_of(a), 0, s, a); return true; }
     }
     GN_LAUNCH((gn_fwd_group_kernel<DT, V, UN, SILU, false>), grid, block_of(a), 0, s, a);
@@ -600,7 +623,7 @@ template <int DT, int V, int UN> bool forward_group(GnArgs a, const Shape& sh, h
 template <int DT, int V, int UN> int forward(GnArgs a, const Shape& sh, void* ws, hipStream_t s) {
     if (forward_group<DT, V, UN>(a, sh, s)) { E3_CHECK_HIP(hipGetLastError()); return E3_OK; }
     GnArgs st = a;
-    map_pass<V>(st, sh, STATS_WGS, 4, false);
+    map_pass<V>(st, sh, STATS_WGS, U1<V>, false);
     st.part = (double*)ws;
     const int units = sh.C / UN, per = st.cg / UN;
     hipLaunchKernelGGL((gn_stats_kernel<DT, V, UN>), grid_of(st), block_of(st), (size_t)st.R * st.PT * (V / UN) * 2 * sizeof(double), s, st);
@@ -608,8 +631,8 @@ template <int DT, int V, int UN> int forward(GnArgs a, const Shape& sh, void* ws
     if ((long long)st.chunks * units <= MERGE_MAX && units <= MERGE_UNITS) { a.rec = st.part; a.rec_chunks = st.chunks; a.rec_units = units; a.rec_per = per; }
     else hipLaunchKernelGGL(gn_finalize_kernel, dim3(sh.N * sh.G), dim3(256), 0, s, st.part, st.chunks, units, per, st.inv_m, a.eps, a.mean_out, a.rstd_out);
     // the checkpoint rides in the apply pass where its blocks are whole there; otherwise it is a pass of its own
-    GnArgs m{}; map_pass<V>(m, sh, APPLY_WGS, 4, true);
-    const bool fused = a.q_out && V == 8 && m.tiles == 1 && m.R * m.PT <= MAX_T && ((unsigned long long)sh.S * sh.C) % CK_BLOCK == 0 && ((uintptr_t)a.q_out & 7) == 0;
+    GnArgs m{}; map_pass<V>(m, sh, APPLY_WGS, U1<V>, true);
+    const bool fused = a.q_out && V > 1 && m.tiles == 1 && m.R * m.PT <= MAX_T && ((unsigned long long)sh.S * sh.C) % CK_BLOCK == 0 && (uintptr_t)a.q_out % V == 0;
     if (a.q_out && !fused) {
         const int rc = launch_checkpoint8_pack(DT, a.x, a.x_ldc, (long long)sh.N * sh.S, sh.C, a.q_out, a.qs_out, s);
         if (rc) return rc;
@@ -622,14 +645,14 @@ template <int DT, int V, int UN> int forward(GnArgs a, const Shape& sh, void* ws
 
 template <int DT, int V, int UN, bool CK> int backward(GnArgs a, const Shape& sh, void* ws, hipStream_t s) {
     GnArgs st = a;
-    map_pass<V>(st, sh, STATS_WGS, 2, false);
+    map_pass<V>(st, sh, STATS_WGS, U2<V>, false);
     st.part = (double*)ws;
     const BwdSpace space = bwd_space(st, sh);
     void* behind = (char*)ws + space.channels;
     if (space.merge) st.gpart = (double*)behind;
     const size_t lds = align_up((size_t)st.R * st.PT * V * 2 * sizeof(float), 8) + (space.merge ? (size_t)sh.C * 2 * sizeof(double) : 0);
     GN_LAUNCH((gn_bwd_reduce_kernel<DT, V, UN, CK, SILU>), grid_of(st), block_of(st), lds, s, st);
-    map_pass<V>(a, sh, APPLY_WGS, 2, false);
+    map_pass<V>(a, sh, APPLY_WGS, U2<V>, false);
     size_t alds = 0;
     const int sums = (a.dgamma || a.dbeta) ? (sh.C + 15) / 16 : 0;
     if (space.merge) {
@@ -650,14 +673,15 @@ template <int DT, int V, int UN, bool CK> int backward(GnArgs a, const Shape& sh
 
 // f(DT, V, UN) as compile-time constants
 template <int I> using Int = std::integral_constant<int, I>;
-template <int DT, typename F> int by_pieces(bool v8, int cg, F f) {
-    if (!v8) return f(Int<DT>(), Int<1>(), Int<1>());
-    if (cg % 8 == 0) return f(Int<DT>(), Int<8>(), Int<8>());
-    if (cg % 4 == 0) return f(Int<DT>(), Int<8>(), Int<4>());
-    return f(Int<DT>(), Int<8>(), Int<1>());
+template <int DT, typename F> int by_pieces(bool wide, int cg, F f) {
+    constexpr int V = wide_of(DT);
+    if (!wide) return f(Int<DT>(), Int<1>(), Int<1>());
+    if (cg % V == 0) return f(Int<DT>(), Int<V>(), Int<V>());
+    if constexpr (V == 8) if (cg % 4 == 0) return f(Int<DT>(), Int<V>(), Int<4>());
+    return f(Int<DT>(), Int<V>(), Int<1>());
 }
-template <typename F> int by_type(int dtype, bool v8, int cg, F f) {
-    return dtype == DT_F32 ? by_pieces<DT_F32>(v8, cg, f) : dtype == DT_BF16 ? by_pieces<DT_BF16>(v8, cg, f) : by_pieces<DT_F16>(v8, cg, f);
+template <typename F> int by_type(int dtype, bool wide, int cg, F f) {
+    return dtype == DT_F32 ? by_pieces<DT_F32>(wide, cg, f) : dtype == DT_BF16 ? by_pieces<DT_BF16>(wide, cg, f) : by_pieces<DT_F16>(wide, cg, f);
 }
 
 bool act_ok(float slope) { return (slope >= 0.f && slope <= 1.f) || slope == ACT_SILU; }
@@ -696,8 +720,8 @@ int e3_group_norm_act_fwd(void* stream, int dtype, const void* x, int x_ldc, con
     GnArgs a{};
     a.x = x; a.x_ldc = x_ldc; a.out = y; a.out_ldc = y_ldc; a.gamma = gamma; a.beta = beta; a.slope = act_slope; a.q_out = q; a.qs_out = q_scale;
     a.eps = eps; a.mean_out = mean; a.rstd_out = rstd;
-    const bool v8 = rows_by_8(dtype, x, x_ldc, C) && rows_by_8(dtype, y, y_ldc, C);
-    return by_type(dtype, v8, C / G, [&](auto dt, auto v, auto un) { return forward<dt.value, v.value, un.value>(a, sh, workspace, (hipStream_t)stream); });
+    const bool wide = wide_rows(dtype, x, x_ldc, C) && wide_rows(dtype, y, y_ldc, C);
+    return by_type(dtype, wide, C / G, [&](auto dt, auto v, auto un) { return forward<dt.value, v.value, un.value>(a, sh, workspace, (hipStream_t)stream); });
 }
 
 int e3_group_norm_act_apply(void* stream, int dtype, const void* x, int x_ldc, const signed char* q, const float* q_scale, const float* mean, const float* rstd,
@@ -709,8 +733,8 @@ int e3_group_norm_act_apply(void* stream, int dtype, const void* x, int x_ldc, c
     E3_REQUIRE((!x || x_ldc >= C) && y_ldc >= C, E3_ERR_INVALID, "rows are shorter than the channel count");
     GnArgs a{};
     a.x = x; a.x_ldc = x_ldc; a.q = q; a.qs = q_scale; a.out = y; a.out_ldc = y_ldc; a.mean = mean; a.rstd = rstd; a.gamma = gamma; a.beta = beta; a.slope = act_slope;
-    const bool v8 = (x ? rows_by_8(dtype, x, x_ldc, C) : C % 8 == 0 && ((uintptr_t)q & 7) == 0) && rows_by_8(dtype, y, y_ldc, C);
-    by_type(dtype, v8, C / G, [&](auto dt, auto v, auto un) {
+    const bool wide = (x ? wide_rows(dtype, x, x_ldc, C) : wide_codes(dtype, q, C)) && wide_rows(dtype, y, y_ldc, C);
+    by_type(dtype, wide, C / G, [&](auto dt, auto v, auto un) {
         if (x) launch_apply<dt.value, v.value, un.value, false>(a, sh, (hipStream_t)stream);
         else launch_apply<dt.value, v.value, un.value, true>(a, sh, (hipStream_t)stream);
         return E3_OK;
@@ -731,8 +755,8 @@ int e3_group_norm_act_bwd(void* stream, int dtype, const void* x, int x_ldc, con
     GnArgs a{};
     a.x = x; a.x_ldc = x_ldc; a.q = q; a.qs = q_scale; a.dy = dy; a.dy_ldc = dy_ldc; a.out = dx; a.out_ldc = dx_ldc;
     a.mean = mean; a.rstd = rstd; a.gamma = gamma; a.beta = beta; a.slope = act_slope; a.dgamma = dgamma; a.dbeta = dbeta;
-    const bool v8 = (x ? rows_by_8(dtype, x, x_ldc, C) : C % 8 == 0 && ((uintptr_t)q & 7) == 0) && rows_by_8(dtype, dy, dy_ldc, C) && rows_by_8(dtype, dx, dx_ldc, C);
-    return by_type(dtype, v8, C / G, [&](auto dt, auto v, auto un) {
+    const bool wide = (x ? wide_rows(dtype, x, x_ldc, C) : wide_codes(dtype, q, C)) && wide_rows(dtype, dy, dy_ldc, C) && wide_rows(dtype, dx, dx_ldc, C);
+    return by_type(dtype, wide, C / G, [&](auto dt, auto v, auto un) {
         return x ? backward<dt.value, v.value, un.value, false>(a, sh, workspace, (hipStream_t)stream)
                  : backward<dt.value, v.value, un.value, true>(a, sh, workspace, (hipStream_t)stream);
     });
