@@ -136,7 +136,7 @@ _SIG = {
     'e3_bn_bwd_workspace_bytes': (c_size_t, [_I, _I, _I, _I, _I]),
     'e3_bn_relu_bwd': (_I, [_P, _P, _I, _P, _P, _P, _P, _P, _P, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I,
                             _P, _I, _P, _P, _P, _P, c_size_t]),
-    'e3_group_norm_workspace_bytes': (c_size_t, [_I, _I, _I, _I, _I, _I]),
+    'e3_group_norm_workspace_bytes': (c_size_t, [_I, _I, _I, _I, _I, _I, _I]),
     'e3_group_norm_act_fwd': (_I, [_P, _I, _P, _I, _P, _P, _F, _F, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P, c_size_t]),
     'e3_group_norm_act_apply': (_I, [_P, _I, _P, _I, _P, _P, _P, _P, _P, _P, _F, _P, _I, _I, _I, _I, _I, _I, _I]),
     'e3_group_norm_act_bwd': (_I, [_P, _I, _P, _I, _P, _P, _P, _P, _P, _P, _F, _P, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P, c_size_t]),

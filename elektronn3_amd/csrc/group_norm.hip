@@ -571,13 +571,28 @@ BwdSpace bwd_space(const GnArgs& a, const Shape& sh) {
     return b;
 }
 size_t max2(size_t a, size_t b) { return a > b ? a : b; }
-template <int V> size_t space_of(const Shape& sh) {
-    GnArgs a{}; map_pass<V>(a, sh, STATS_WGS, U2<V>, false);
-    const BwdSpace b = bwd_space(a, sh);
-    return max2(fwd_part_doubles<V>(sh) * sizeof(double), b.channels + b.behind);
+// One workgroup per group where the pieces of a bundle fit its threads' registers: fills in PT and R
+template <int V> bool map_group(GnArgs& a, const Shape& sh) {
+    set_shape(a, sh);
+    if (a.cg % V != 0 && V % a.cg != 0) return false;
+    a.P = sh.C / V;
+    a.PT = a.cg > V ? a.cg / V : 1;
+    if (a.PT > MAX_T || sh.S > (long long)HELD<V> * (MAX_T / a.PT)) return false;
+    a.R = MAX_T / a.PT;
+    for (int t = MAX_T / 2; t >= 64; t /= 2)             // no more threads than pieces
+        if (t / a.PT > 0 && sh.S <= t / a.PT) a.R = t / a.PT;
+    return true;
 }
-size_t workspace_bytes(const Shape& sh) {      // (for every type and alignment)
-    return max2(space_of<1>(sh), max2(sh.C % 4 == 0 ? space_of<4>(sh) : 0, sh.C % 8 == 0 ? space_of<8>(sh) : 0));
+template <int V> size_t space_of(const Shape& sh, bool backward) {
+    if (sh.C % V != 0) return 0;
+    GnArgs a{};
+    if (!backward) return map_group<V>(a, sh) ? 0 : fwd_part_doubles<V>(sh) * sizeof(double);
+    map_pass<V>(a, sh, STATS_WGS, U2<V>, false);
+    const BwdSpace b = bwd_space(a, sh);
+    return b.channels + b.behind;
+}
+size_t workspace_bytes(const Shape& sh, bool backward) {      // (for every type and alignment)
+    return max2(space_of<1>(sh, backward), max2(space_of<4>(sh, backward), space_of<8>(sh, backward)));
 }
 size_t merge_lds(const GnArgs& a, int units) { return (size_t)2 * (block_of(a).x + units) * sizeof(double); }
 
@@ -597,31 +612,25 @@ template <int DT, int V, int UN, bool CK> void launch_apply(GnArgs a, const Shap
     GN_LAUNCH((gn_apply_kernel<DT, V, UN, CK, SILU, false>), grid_of(a), block_of(a), lds, s, a);
 }
 
-// One workgroup per group where the pieces of a bundle fit its threads' registers
-template <int DT, int V, int UN> bool forward_group(GnArgs a, const Shape& sh, hipStream_t s) {
-#ifdef GN_GROUP_OFF
-    return false;
-#endif
-    set_shape(a, sh);
-    if (a.cg % V != 0 && V % a.cg != 0) return false;
-    a.P = sh.C / V;
-    a.PT = a.cg > V ? a.cg / V : 1;
-    if (a.PT > MAX_T || sh.S > (long long)HELD<V> * (MAX_T / a.PT)) return false;
-    const bool keep = a.q_out != nullptr;
-    if (keep && !(V > 1 && a.PT * V % CK_BLOCK == 0 && (uintptr_t)a.q_out % V == 0)) return false;
-    a.R = MAX_T / a.PT;
-    for (int t = MAX_T / 2; t >= 64; t /= 2)             // no more threads than pieces
-        if (t / a.PT > 0 && sh.S <= t / a.PT) a.R = t / a.PT;
+template <int DT, int V, int UN> int forward_group(GnArgs a, const Shape& sh, hipStream_t s) {
     const dim3 grid((unsigned)((long long)sh.N * (a.P / a.PT)));
     if constexpr (V > 1 && UN == V) {
-        if (keep) { GN_LAUNCH((gn_fwd_group_kernel<DT, V, UN, SILU, true>), grid, block_of(a), 0, s, a); return true; }
+        if (a.q_out && a.PT * V % CK_BLOCK == 0 && (uintptr_t)a.q_out % V == 0) {      // bundles of whole blocks
+            GN_LAUNCH((gn_fwd_group_kernel<DT, V, UN, SILU, true>), grid, block_of(a), 0, s, a);
+            return E3_OK;
+        }
     }
+    if (a.q_out) { const int rc = launch_checkpoint8_pack(DT, a.x, a.x_ldc, (long long)sh.N * sh.S, sh.C, a.q_out, a.qs_out, s); if (rc) return rc; }
     GN_LAUNCH((gn_fwd_group_kernel<DT, V, UN, SILU, false>), grid, block_of(a), 0, s, a);
-    return true;
+    return E3_OK;
 }
 
 template <int DT, int V, int UN> int forward(GnArgs a, const Shape& sh, void* ws, hipStream_t s) {
-    if (forward_group<DT, V, UN>(a, sh, s)) { E3_CHECK_HIP(hipGetLastError()); return E3_OK; }
+    if (map_group<V>(a, sh)) {
+        const int rc = forward_group<DT, V, UN>(a, sh, s);
+        E3_CHECK_HIP(hipGetLastError());
+        return rc;
+    }
     GnArgs st = a;
     map_pass<V>(st, sh, STATS_WGS, U1<V>, false);
     st.part = (double*)ws;
@@ -701,10 +710,10 @@ int check_shape(int dtype, int N, int D, int H, int W, int C, int G, float slope
 
 extern "C" {
 
-size_t e3_group_norm_workspace_bytes(int N, int D, int H, int W, int C, int G) {
+size_t e3_group_norm_workspace_bytes(int N, int D, int H, int W, int C, int G, int backward) {
     Shape sh;
     if (check_shape(0, N, D, H, W, C, G, 0.f, sh)) return 0;
-    return workspace_bytes(sh);
+    return workspace_bytes(sh, backward != 0);
 }
 
 int e3_group_norm_act_fwd(void* stream, int dtype, const void* x, int x_ldc, const float* gamma, const float* beta, float eps, float act_slope, void* y, int y_ldc,
@@ -712,11 +721,12 @@ int e3_group_norm_act_fwd(void* stream, int dtype, const void* x, int x_ldc, con
     Shape sh;
     const int rc = check_shape(dtype, N, D, H, W, C, G, act_slope, sh);
     if (rc) return rc;
-    E3_REQUIRE(x && y && mean && rstd && workspace, E3_ERR_INVALID, "null argument");
+    E3_REQUIRE(x && y && mean && rstd, E3_ERR_INVALID, "null argument");
     E3_REQUIRE((q == nullptr) == (q_scale == nullptr), E3_ERR_INVALID, "a checkpoint is codes and scales");
     E3_REQUIRE(x_ldc >= C && y_ldc >= C, E3_ERR_INVALID, "rows are shorter than the channel count");
     E3_REQUIRE(eps >= 0.f, E3_ERR_INVALID, "eps must not be negative");
-    E3_REQUIRE(workspace_bytes_ >= workspace_bytes(sh), E3_ERR_WORKSPACE, "workspace too small");
+    const size_t need = workspace_bytes(sh, false);
+    E3_REQUIRE(workspace_bytes_ >= need && (workspace || !need), E3_ERR_WORKSPACE, "workspace too small");
     GnArgs a{};
     a.x = x; a.x_ldc = x_ldc; a.out = y; a.out_ldc = y_ldc; a.gamma = gamma; a.beta = beta; a.slope = act_slope; a.q_out = q; a.qs_out = q_scale;
     a.eps = eps; a.mean_out = mean; a.rstd_out = rstd;
@@ -751,7 +761,7 @@ int e3_group_norm_act_bwd(void* stream, int dtype, const void* x, int x_ldc, con
     if (rc) return rc;
     E3_REQUIRE(dy && dx && mean && rstd && workspace && (x || (q && q_scale)), E3_ERR_INVALID, "null argument");
     E3_REQUIRE((!x || x_ldc >= C) && dy_ldc >= C && dx_ldc >= C, E3_ERR_INVALID, "rows are shorter than the channel count");
-    E3_REQUIRE(workspace_bytes_ >= workspace_bytes(sh), E3_ERR_WORKSPACE, "workspace too small");
+    E3_REQUIRE(workspace_bytes_ >= workspace_bytes(sh, true), E3_ERR_WORKSPACE, "workspace too small");
     GnArgs a{};
     a.x = x; a.x_ldc = x_ldc; a.q = q; a.qs = q_scale; a.dy = dy; a.dy_ldc = dy_ldc; a.out = dx; a.out_ldc = dx_ldc;
     a.mean = mean; a.rstd = rstd; a.gamma = gamma; a.beta = beta; a.slope = act_slope; a.dgamma = dgamma; a.dbeta = dbeta;

@@ -427,6 +427,10 @@ class Checkpoint8:
         return f'Checkpoint8(shape={tuple(self.shape)}, dtype={self.dtype}, device={self.device})'
 
 
+def _like(x):
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
 def _new_checkpoint(x):
     n = x.numel()
     ck = Checkpoint8.__new__(Checkpoint8)
@@ -503,18 +507,18 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, activation='
     if not eps >= 0:
         raise ValueError('eps must not be negative')
     if out is None:
-        y, y_ldc = torch.empty(shape, dtype=dtype, device=device), C
+        y, y_ldc = _like(x), C
     else:
         y, y_ldc = out, _chk_any(out, 'out', shape, dtype, device)
         _chk_out(out, x)
     L = _lib.load()
     mean = torch.empty((dims[0], num_groups), dtype=torch.float32, device=device)
-    rstd = torch.empty((dims[0], num_groups), dtype=torch.float32, device=device)
+    rstd = torch.empty_like(mean)
     ck = _new_checkpoint(x) if checkpoint else None
-    nbytes = L.e3_group_norm_workspace_bytes(*dims)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    nbytes = L.e3_group_norm_workspace_bytes(*dims, 0)           # (0 for small groups)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
     _call(device, L.e3_group_norm_act_fwd, _DT[dtype], x.data_ptr(), ldc, wp, bp, eps, slope, y.data_ptr(), y_ldc, mean.data_ptr(), rstd.data_ptr(),
-          ck.q.data_ptr() if ck else None, ck.scale.data_ptr() if ck else None, *dims, ws.data_ptr(), nbytes)
+          ck.q.data_ptr() if ck else None, ck.scale.data_ptr() if ck else None, *dims, ws.data_ptr() if nbytes else None, nbytes)
     return (y, mean, rstd, ck) if checkpoint else (y, mean, rstd)
 
 
@@ -529,7 +533,7 @@ def group_norm_act_apply(x, mean, rstd, weight=None, bias=None, activation='relu
     C = dims[4]
     weight, bias, wp, bp = _affine(weight, bias, C, device)
     if out is None:
-        y, y_ldc = torch.empty(shape, dtype=dtype, device=device), C
+        y, y_ldc = torch.empty(shape, dtype=dtype, device=device) if src[0] is None else _like(x), C
     else:
         y, y_ldc = out, _chk_any(out, 'out', shape, dtype, device)
         if src[0] is not None:
@@ -550,10 +554,10 @@ def group_norm_act_bwd(x, mean, rstd, dy, weight=None, bias=None, activation='re
     weight, bias, wp, bp = _affine(weight, bias, C, device)
     dy_ldc = _chk_any(dy, 'dy', shape, dtype, device)
     L = _lib.load()
-    dx = torch.empty(shape, dtype=dtype, device=device)
+    dx = _like(dy)
     dw = torch.empty(C, dtype=torch.float32, device=device)
-    db = torch.empty(C, dtype=torch.float32, device=device)
-    nbytes = L.e3_group_norm_workspace_bytes(*dims)
+    db = torch.empty_like(dw)
+    nbytes = L.e3_group_norm_workspace_bytes(*dims, 1)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
     _call(device, L.e3_group_norm_act_bwd, _DT[dtype], *src, mean.data_ptr(), rstd.data_ptr(), wp, bp, slope, dy.data_ptr(), dy_ldc, dx.data_ptr(), C,
           dw.data_ptr(), db.data_ptr(), *dims, ws.data_ptr(), nbytes)

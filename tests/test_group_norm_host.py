@@ -65,7 +65,7 @@ def test_module_arguments():
 
 
 # the C ABI: (N, D, H, W, C, G) that are no sizes, types, slopes, rows, workspaces
-GOOD = (2, 3, 4, 5, 16, 4)
+GOOD = (2, 30, 40, 50, 16, 4)        # (large enough to need a workspace)
 
 
 def fwd(dtype=0, x=FAKE, x_ldc=16, eps=1e-5, slope=0.0, y=FAKE, y_ldc=16, mean=FAKE, q=None, qs=None, dims=GOOD, ws=FAKE, nbytes=0):
@@ -73,7 +73,7 @@ def fwd(dtype=0, x=FAKE, x_ldc=16, eps=1e-5, slope=0.0, y=FAKE, y_ldc=16, mean=F
 
 
 @pytest.mark.parametrize('kw,code', [
-    (dict(dtype=3), 1), (dict(dtype=-1), 1), (dict(x=None), 1), (dict(y=None), 1), (dict(mean=None), 1), (dict(ws=None), 1), (dict(x_ldc=15), 1), (dict(y_ldc=8), 1),
+    (dict(dtype=3), 1), (dict(dtype=-1), 1), (dict(x=None), 1), (dict(y=None), 1), (dict(mean=None), 1), (dict(ws=None, nbytes=1 << 30), 4), (dict(x_ldc=15), 1), (dict(y_ldc=8), 1),
     (dict(eps=-1.0), 1), (dict(eps=float('nan')), 1), (dict(slope=3.0), 3), (dict(slope=-0.5), 3), (dict(slope=float('nan')), 3), (dict(q=FAKE), 1), (dict(qs=FAKE), 1),
     (dict(dims=(2, 3, 4, 5, 16, 3)), 1), (dict(dims=(2, 3, 4, 5, 16, 0)), 1), (dict(dims=(0, 3, 4, 5, 16, 4)), 1), (dict(dims=(2, 0, 4, 5, 16, 4)), 1),
     (dict(dims=(2, 3, 4, 5, 0, 4)), 1), (dict(), 4), (dict(nbytes=64), 4)])
@@ -105,6 +105,8 @@ def test_checkpoint_refusals():
 
 @pytest.mark.parametrize('dims', [GOOD, (1, 1, 1, 1, 8, 1), (3, 17, 45, 51, 20, 5), (2, 64, 128, 128, 32, 8), (1, 1, 1, 1, 8192, 8192), (100000, 1, 1, 1, 8, 8), (1, 2048, 2048, 2048, 8, 8)])
 def test_workspace_sizes(dims):
-    n = call('e3_group_norm_workspace_bytes', *dims)
-    assert 0 < n < 1 << 31
-    assert call('e3_group_norm_workspace_bytes', *dims[:5], dims[5] + dims[4] + 1) == 0
+    assert 0 <= call('e3_group_norm_workspace_bytes', *dims, 0) < 1 << 31
+    assert 0 < call('e3_group_norm_workspace_bytes', *dims, 1) < 1 << 31
+    assert call('e3_group_norm_workspace_bytes', *dims[:5], dims[5] + dims[4] + 1, 1) == 0
+    # the forward of small groups needs none
+    assert call('e3_group_norm_workspace_bytes', 1, 4, 8, 8, 128, 8, 0) == 0 < call('e3_group_norm_workspace_bytes', 1, 64, 64, 64, 128, 8, 0)
