@@ -39,11 +39,12 @@ template <> struct Raw<DT_F32, 4> { f32x4 v; };
 template <> struct Raw<DT_BF16, 8> { u16x8 v; };
 template <> struct Raw<DT_F16, 8> { u16x8 v; };
 
-template <int DT, int V> __device__ __forceinline__ Raw<DT, V> load_raw(const typename Elem<DT>::T* p) {
+// NT: non-temporal, for data that nobody reads again
+template <int DT, int V, bool NT = false> __device__ __forceinline__ Raw<DT, V> load_raw(const typename Elem<DT>::T* p) {
+    typedef decltype(Raw<DT, V>::v) P;
     Raw<DT, V> r;
-    if constexpr (V == 1) r.v = *p;
-    else if constexpr (DT == DT_F32) r.v = *reinterpret_cast<const f32x4*>(p);
-    else r.v = *reinterpret_cast<const u16x8*>(p);
+    if constexpr (NT) r.v = __builtin_nontemporal_load(reinterpret_cast<const P*>(p));
+    else r.v = *reinterpret_cast<const P*>(p);
     return r;
 }
 template <int DT, int V> __device__ __forceinline__ void unpack_raw(const Raw<DT, V>& r, float (&f)[V]) {
@@ -56,16 +57,16 @@ template <int DT, int V> __device__ __forceinline__ void unpack_raw(const Raw<DT
         for (int e = 0; e < 8; ++e) f[e] = to_f32<DT>(r.v[e]);
     }
 }
-template <int DT, int V> __device__ __forceinline__ void store_f32(typename Elem<DT>::T* p, const float (&f)[V]) {
-    if constexpr (V == 1) *p = from_f32<DT>(f[0]);
-    else if constexpr (DT == DT_F32) {
-        *reinterpret_cast<f32x4*>(p) = f32x4{f[0], f[1], f[2], f[3]};
-    } else {
-        u16x8 o;
+template <int DT, int V, bool NT = false> __device__ __forceinline__ void store_f32(typename Elem<DT>::T* p, const float (&f)[V]) {
+    typedef decltype(Raw<DT, V>::v) P;
+    P o;
+    if constexpr (V == 1) o = from_f32<DT>(f[0]);
+    else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = from_f32<DT>(f[e]);
-        *reinterpret_cast<u16x8*>(p) = o;
+        for (int e = 0; e < V; ++e) o[e] = from_f32<DT>(f[e]);
     }
+    if constexpr (NT) __builtin_nontemporal_store(o, reinterpret_cast<P*>(p));
+    else *reinterpret_cast<P*>(p) = o;
 }
 
 // V codes of a checkpoint and their scale

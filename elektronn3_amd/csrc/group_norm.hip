@@ -68,12 +68,12 @@ template <int V> __device__ __forceinline__ Where where(const GnArgs& a, unsigne
 }
 
 // one piece of the input
-template <int DT, int V, bool CK> struct In {
+template <int DT, int V, bool CK, bool NT = false> struct In {
     Raw<DT, V> r;
-    __device__ __forceinline__ void load(const GnArgs& a, long long row, int c) { r = load_raw<DT, V>((const typename Elem<DT>::T*)a.x + (size_t)row * a.x_ldc + c); }
+    __device__ __forceinline__ void load(const GnArgs& a, long long row, int c) { r = load_raw<DT, V, NT>((const typename Elem<DT>::T*)a.x + (size_t)row * a.x_ldc + c); }
     __device__ __forceinline__ void get(float (&f)[V]) const { unpack_raw<DT, V>(r, f); }
 };
-template <int DT, int V> struct In<DT, V, true> {
+template <int DT, int V, bool NT> struct In<DT, V, true, NT> {
     RawQ<V> r;
     __device__ __forceinline__ void load(const GnArgs& a, long long row, int c) { r = load_q<V>(a.q, a.qs, (size_t)row * a.C + c); }
     __device__ __forceinline__ void get(float (&f)[V]) const { unpack_q<V>(r, f); }
@@ -219,13 +219,16 @@ __global__ __launch_bounds__(MAX_T) void gn_stats_kernel(const GnArgs a) {
     sum_rows(sh, s2, a.R, units, [&](int u, double x, double y) { if (first + u < all) { o[(first + u) * 2] = x; o[(first + u) * 2 + 1] = y; } });
 }
 
-template <int DT, int V, int UN, bool CK, bool SILU, bool KEEP>
+// NT: the input is read for the last time and the output written past the caches (non-temporal), which leaves the memory-side cache to what the statistics or
+// reduce pass has just read: forward of 2 x 64 x 128 x 128 x 32 in fp32 168 -> 130 us, in bf16 92 -> 72, a pass from the checkpoint 84 -> 54; with the next reader of y
+// timed along 233 -> 217, 133 -> 118, at 34 MB 38.2 -> 36.8.  From a tensor that no pass has read before it loses (bf16 53 -> 58): not there.
+template <int DT, int V, int UN, bool CK, bool SILU, bool KEEP, bool NT>
 __global__ __launch_bounds__(MAX_T) void gn_apply_kernel(const GnArgs a) {
     extern __shared__ double sh[];
     const Where w = where<V>(a, blockIdx.x);
     constexpr int U = U1<V>;
     typedef typename Elem<DT>::T T;
-    In<DT, V, CK> in[U]; bool ok[U];
+    In<DT, V, CK, NT> in[U]; bool ok[U];
     auto load = [&](long long vb) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -265,7 +268,7 @@ __global__ __launch_bounds__(MAX_T) void gn_apply_kernel(const GnArgs a) {
             }
 #pragma unroll
             for (int e = 0; e < V; ++e) o[e] = activate<SILU>(__builtin_fmaf(f[e] - k.mu[e / UN], k.a[e], k.b[e]), a.slope);
-            if (ok[u]) store_f32<DT, V>((T*)a.out + row * a.out_ldc + w.c, o);
+            if (ok[u]) store_f32<DT, V, NT>((T*)a.out + row * a.out_ldc + w.c, o);
         }
         vb -= step;
         if (vb < w.v0) break;
@@ -478,14 +481,15 @@ __global__ __launch_bounds__(MAX_T) void gn_bwd_apply_kernel(const GnArgs a) {
     const Where w = where<V>(a, blockIdx.x - a.sum_wgs);
     constexpr int U = U2<V>;
     typedef typename Elem<DT>::T T;
-    In<DT, V, CK> in[U]; Raw<DT, V> dy[U]; bool ok[U];
+    constexpr bool NT = V > 1;               // (as in the forward: 255 -> 230 us, bf16 131 -> 115)
+    In<DT, V, CK, NT> in[U]; Raw<DT, V> dy[U]; bool ok[U];
     auto load = [&](long long vb) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const long long v = vb + w.r + u * a.R, row = w.n * a.S + v;
             ok[u] = w.on && v < w.v1;
             in[u].r = {}; dy[u] = {};
-            if (ok[u]) { in[u].load(a, row, w.c); dy[u] = load_raw<DT, V>((const T*)a.dy + (size_t)row * a.dy_ldc + w.c); }
+            if (ok[u]) { in[u].load(a, row, w.c); dy[u] = load_raw<DT, V, NT>((const T*)a.dy + (size_t)row * a.dy_ldc + w.c); }
         }
     };
     const int step = U * a.R;                // (from the end, as in the forward)
@@ -510,7 +514,7 @@ __global__ __launch_bounds__(MAX_T) void gn_bwd_apply_kernel(const GnArgs a) {
             grad_piece<V, UN, SILU>(a, w.n, w.c, f, g, k, border, dz, d);
 #pragma unroll
             for (int e = 0; e < V; ++e) o[e] = __builtin_fmaf(k.a[e], dz[e], -__builtin_fmaf(d[e], c2[e / UN], c1[e / UN]));
-            if (ok[u]) store_f32<DT, V>((T*)a.out + (size_t)(w.n * a.S + vb + w.r + u * a.R) * a.out_ldc + w.c, o);
+            if (ok[u]) store_f32<DT, V, NT>((T*)a.out + (size_t)(w.n * a.S + vb + w.r + u * a.R) * a.out_ldc + w.c, o);
         }
         vb -= step;
         if (vb < w.v0) break;
@@ -521,12 +525,8 @@ __global__ __launch_bounds__(MAX_T) void gn_bwd_apply_kernel(const GnArgs a) {
 // ------------------------------------------------------------------------------------------------ host side
 struct Shape { int N; long long S; int C, G; };
 
-#ifndef GN_STATS_WGS
-#define GN_STATS_WGS 512
-#define GN_APPLY_WGS 512
-#define GN_BT 256
-#endif
-constexpr int STATS_WGS = GN_STATS_WGS, APPLY_WGS = GN_APPLY_WGS;
+constexpr int PASS_WGS = 512;                // workgroups of a pass: two per CU (256 threads each); 1024 cost the merges of mid-sized tensors 2 - 8 us and gain nothing
+constexpr int PASS_T = 256;
 
 void set_shape(GnArgs& a, const Shape& sh) { a.N = sh.N; a.S = sh.S; a.C = sh.C; a.G = sh.G; a.cg = sh.C / sh.G; a.inv_m = 1.0 / ((double)sh.S * a.cg); }
 
@@ -536,7 +536,7 @@ template <int V> void map_pass(GnArgs& a, const Shape& sh, int target, int U, bo
     a.P = sh.C / V;
     a.tiles = (a.P + MAX_T - 1) / MAX_T;
     a.PT = (a.P + a.tiles - 1) / a.tiles;
-    a.R = GN_BT / a.PT > 0 ? GN_BT / a.PT : 1;
+    a.R = PASS_T / a.PT > 0 ? PASS_T / a.PT : 1;
     if (keep) {                              // whole blocks of 64 elements per workgroup step
         int k = CK_BLOCK / V;
         for (int p = a.PT; k > 1 && p % 2 == 0; p /= 2) k /= 2;
@@ -558,7 +558,7 @@ dim3 block_of(const GnArgs& a) { return dim3((unsigned)((a.R * a.PT + 63) / 64 *
 int unit_of(int V, int cg) { return V >= 8 && cg % 8 == 0 ? 8 : V >= 4 && cg % 4 == 0 ? 4 : 1; }
 
 template <int V> size_t fwd_part_doubles(const Shape& sh) {
-    GnArgs a{}; map_pass<V>(a, sh, STATS_WGS, U1<V>, false);
+    GnArgs a{}; map_pass<V>(a, sh, PASS_WGS, U1<V>, false);
     return (size_t)sh.N * a.chunks * (sh.C / unit_of(V, sh.C / sh.G)) * 2;
 }
 // what lies in the workspace of a backward pass: channel records, then group records (`merge`) or m1 and m2
@@ -587,7 +587,7 @@ template <int V> size_t space_of(const Shape& sh, bool backward) {
     if (sh.C % V != 0) return 0;
     GnArgs a{};
     if (!backward) return map_group<V>(a, sh) ? 0 : fwd_part_doubles<V>(sh) * sizeof(double);
-    map_pass<V>(a, sh, STATS_WGS, U2<V>, false);
+    map_pass<V>(a, sh, PASS_WGS, U2<V>, false);
     const BwdSpace b = bwd_space(a, sh);
     return b.channels + b.behind;
 }
@@ -602,14 +602,17 @@ size_t merge_lds(const GnArgs& a, int units) { return (size_t)2 * (block_of(a).x
         else { constexpr bool SILU = false; hipLaunchKernelGGL((KERNEL), GRID, BLOCK, LDS, S, A); }                                     \
     } while (0)
 
-template <int DT, int V, int UN, bool CK> void launch_apply(GnArgs a, const Shape& sh, hipStream_t s) {
+// BEHIND: behind a statistics pass of the same call
+template <int DT, int V, int UN, bool CK, bool BEHIND> void launch_apply(GnArgs a, const Shape& sh, hipStream_t s) {
     const bool keep = a.q_out != nullptr;
-    map_pass<V>(a, sh, APPLY_WGS, U1<V>, keep);
+    // (merging the records costs a workgroup 1 - 2 us: twice the workgroups without it, 74 -> 53 us for 2 x 64 x 128 x 128 x 32 in bf16)
+    map_pass<V>(a, sh, a.rec ? PASS_WGS : 2 * PASS_WGS, U1<V>, keep);
     const size_t lds = a.rec ? merge_lds(a, a.rec_units) : 0;
-    if constexpr (V > 1 && !CK) {
-        if (keep) { GN_LAUNCH((gn_apply_kernel<DT, V, UN, CK, SILU, true>), grid_of(a), block_of(a), lds, s, a); return; }
+    constexpr bool NT = V > 1 && (BEHIND || CK);
+    if constexpr (V > 1 && BEHIND) {
+        if (keep) { GN_LAUNCH((gn_apply_kernel<DT, V, UN, CK, SILU, true, NT>), grid_of(a), block_of(a), lds, s, a); return; }
     }
-    GN_LAUNCH((gn_apply_kernel<DT, V, UN, CK, SILU, false>), grid_of(a), block_of(a), lds, s, a);
+    GN_LAUNCH((gn_apply_kernel<DT, V, UN, CK, SILU, false, NT>), grid_of(a), block_of(a), lds, s, a);
 }
 
 template <int DT, int V, int UN> int forward_group(GnArgs a, const Shape& sh, hipStream_t s) {
@@ -632,7 +635,7 @@ template <int DT, int V, int UN> int forward(GnArgs a, const Shape& sh, void* ws
         return rc;
     }
     GnArgs st = a;
-    map_pass<V>(st, sh, STATS_WGS, U1<V>, false);
+    map_pass<V>(st, sh, PASS_WGS, U1<V>, false);
     st.part = (double*)ws;
     const int units = sh.C / UN, per = st.cg / UN;
     hipLaunchKernelGGL((gn_stats_kernel<DT, V, UN>), grid_of(st), block_of(st), (size_t)st.R * st.PT * (V / UN) * 2 * sizeof(double), s, st);
@@ -640,28 +643,28 @@ template <int DT, int V, int UN> int forward(GnArgs a, const Shape& sh, void* ws
     if ((long long)st.chunks * units <= MERGE_MAX && units <= MERGE_UNITS) { a.rec = st.part; a.rec_chunks = st.chunks; a.rec_units = units; a.rec_per = per; }
     else hipLaunchKernelGGL(gn_finalize_kernel, dim3(sh.N * sh.G), dim3(256), 0, s, st.part, st.chunks, units, per, st.inv_m, a.eps, a.mean_out, a.rstd_out);
     // the checkpoint rides in the apply pass where its blocks are whole there; otherwise it is a pass of its own
-    GnArgs m{}; map_pass<V>(m, sh, APPLY_WGS, U1<V>, true);
+    GnArgs m{}; map_pass<V>(m, sh, PASS_WGS, U1<V>, true);
     const bool fused = a.q_out && V > 1 && m.tiles == 1 && m.R * m.PT <= MAX_T && ((unsigned long long)sh.S * sh.C) % CK_BLOCK == 0 && (uintptr_t)a.q_out % V == 0;
     if (a.q_out && !fused) {
         const int rc = launch_checkpoint8_pack(DT, a.x, a.x_ldc, (long long)sh.N * sh.S, sh.C, a.q_out, a.qs_out, s);
         if (rc) return rc;
         a.q_out = nullptr;
     }
-    launch_apply<DT, V, UN, false>(a, sh, s);
+    launch_apply<DT, V, UN, false, true>(a, sh, s);
     E3_CHECK_HIP(hipGetLastError());
     return E3_OK;
 }
 
 template <int DT, int V, int UN, bool CK> int backward(GnArgs a, const Shape& sh, void* ws, hipStream_t s) {
     GnArgs st = a;
-    map_pass<V>(st, sh, STATS_WGS, U2<V>, false);
+    map_pass<V>(st, sh, PASS_WGS, U2<V>, false);
     st.part = (double*)ws;
     const BwdSpace space = bwd_space(st, sh);
     void* behind = (char*)ws + space.channels;
     if (space.merge) st.gpart = (double*)behind;
     const size_t lds = align_up((size_t)st.R * st.PT * V * 2 * sizeof(float), 8) + (space.merge ? (size_t)sh.C * 2 * sizeof(double) : 0);
     GN_LAUNCH((gn_bwd_reduce_kernel<DT, V, UN, CK, SILU>), grid_of(st), block_of(st), lds, s, st);
-    map_pass<V>(a, sh, APPLY_WGS, U2<V>, false);
+    map_pass<V>(a, sh, PASS_WGS, U2<V>, false);
     size_t alds = 0;
     const int sums = (a.dgamma || a.dbeta) ? (sh.C + 15) / 16 : 0;
     if (space.merge) {
@@ -745,8 +748,8 @@ int e3_group_norm_act_apply(void* stream, int dtype, const void* x, int x_ldc, c
     a.x = x; a.x_ldc = x_ldc; a.q = q; a.qs = q_scale; a.out = y; a.out_ldc = y_ldc; a.mean = mean; a.rstd = rstd; a.gamma = gamma; a.beta = beta; a.slope = act_slope;
     const bool wide = (x ? wide_rows(dtype, x, x_ldc, C) : wide_codes(dtype, q, C)) && wide_rows(dtype, y, y_ldc, C);
     by_type(dtype, wide, C / G, [&](auto dt, auto v, auto un) {
-        if (x) launch_apply<dt.value, v.value, un.value, false>(a, sh, (hipStream_t)stream);
-        else launch_apply<dt.value, v.value, un.value, true>(a, sh, (hipStream_t)stream);
+        if (x) launch_apply<dt.value, v.value, un.value, false, false>(a, sh, (hipStream_t)stream);
+        else launch_apply<dt.value, v.value, un.value, true, false>(a, sh, (hipStream_t)stream);
         return E3_OK;
     });
     E3_CHECK_HIP(hipGetLastError());
