@@ -555,6 +555,13 @@ __global__ void gn_bwd_coef_kernel(const float* __restrict__ dgamma, const float
     coef[3 * C + c] = (float)(m2 * f);
 }
 
+// blockIdx.y = job
+struct CopyJobs { CopyJob j[32]; };
+__global__ void copy_multi_kernel(const CopyJobs jobs) {
+    const CopyJob j = jobs.j[blockIdx.y];
+    for (size_t i = blockIdx.x * (size_t)blockDim.x + threadIdx.x; i < j.n; i += (size_t)gridDim.x * blockDim.x) j.dst[i] = j.src[i];
+}
+
 __global__ void colsum_finalize_kernel(const float* __restrict__ part, int parts, int part_stride, int offset, int C, float* out) {
     const int lane = threadIdx.x & 63;
     const int c = blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6);
@@ -1013,6 +1020,18 @@ __global__ __launch_bounds__(256) void prelu_dslope_kernel(const float* __restri
 }
 int launch_prelu_dslope(const float* part, int parts, int C, float* tmp, float* dslope, hipStream_t s) {
     hipLaunchKernelGGL(prelu_dslope_kernel, dim3(1), dim3(256), 0, s, part, parts, C, tmp, dslope);
+    E3_CHECK_HIP(hipGetLastError());
+    return E3_OK;
+}
+
+int launch_copy_multi(const CopyJob* jobs, int count, hipStream_t s) {
+    for (int at = 0; at < count; at += 32) {
+        CopyJobs a{};
+        const int m = count - at < 32 ? count - at : 32;
+        size_t most = 1;
+        for (int i = 0; i < m; ++i) { a.j[i] = jobs[at + i]; if (jobs[at + i].n > most) most = jobs[at + i].n; }
+        hipLaunchKernelGGL(copy_multi_kernel, dim3(ew_grid(most), m), dim3(EW_BLOCK), 0, s, a);
+    }
     E3_CHECK_HIP(hipGetLastError());
     return E3_OK;
 }

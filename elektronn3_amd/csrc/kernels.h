@@ -219,6 +219,8 @@ struct ColsumJob { const float* part; int parts, stride, offset, C; float* out; 
 int launch_colsum_multi(const ColsumJob* jobs, int njobs, hipStream_t s);   // out[c] = sum_p part[p*stride + offset + c], many at once
 // PReLU: dslope[0] = sum over channels and partial rows of row 2 of the REDUCE pass' `part` (fixed order); tmp: [C] floats
 int launch_prelu_dslope(const float* part, int parts, int C, float* tmp, float* dslope, hipStream_t s);
+struct CopyJob { const float* src; float* dst; size_t n; };
+int launch_copy_multi(const CopyJob* jobs, int count, hipStream_t s);      // small tensors, up to 32 per launch
 int launch_gn_bwd_coef(const float* dgamma, const float* dbeta, const float* gamma, const float* invstd, int C, int group, float inv_n,
                        float* coef, hipStream_t s);   // GroupNorm: rewrites coef after launch_bn_bwd_finalize
 int launch_fill(float* p, float v, size_t n, hipStream_t s);

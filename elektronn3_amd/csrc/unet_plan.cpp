@@ -16,6 +16,7 @@
 #include <unordered_map>
 #include <vector>
 
+#include "checkpoint8.h"
 #include "plan_internal.h"
 
 namespace {
@@ -670,6 +671,97 @@ int e3_unet_sizes(const e3_unet_plan* plan, int N, int D, int H, int W, int trai
     plan_buffers(plan, N, D, H, W, training != 0, nullptr, nullptr, B);
     if (saved_bytes) *saved_bytes = B.saved_bytes;
     if (scratch_bytes) *scratch_bytes = B.scratch_bytes;
+    return E3_OK;
+}
+
+// ---- the saved activations in 8 bits between the passes (e3_unet_checkpoint8_*) --------------------------------------------------------------
+// Of a unit with a norm only its raw tensor (the norm's input) cannot be formed again from the others: it is kept as an 8-bit checkpoint beside the norm's
+// four [C] vectors; the activation, the pooled tensor, the halves of the concat buffer and their sum are recomputed from the restored raw tensors.
+namespace {
+struct Kept8 {
+    std::vector<signed char*> q; std::vector<float*> scale; std::vector<float*> vec;
+    float* xin = nullptr; size_t xin_floats = 0;
+    size_t bytes = 0;
+};
+bool checkpoint8_covered(const e3_unet_plan* p) {
+    if (p->cfg.attention || p->cfg.resunet || p->cfg.conv_valid || p->cfg.up_resize) return false;
+    for (const ConvUnit& u : p->units) if (!u.has_norm()) return false;
+    return true;
+}
+size_t unit_elems(const NetDims& ND, const e3_unet_plan* p, size_t k) { return ND.u[k].out.vox * (size_t)p->units[k].cout; }
+size_t vec_floats(int C) { return 3 * (align_up((size_t)C * sizeof(float), 256) / sizeof(float)) + C; }      // mean .. shift as plan_buffers lays them out
+void kept8_layout(const e3_unet_plan* p, const NetDims& ND, void* base, Kept8& K) {
+    Arena A(base);
+    if (p->cfg.in_channels > 1) { K.xin_floats = ND.X[0].vox * p->cfg.in_channels; K.xin = A.take(K.xin_floats); }
+    for (size_t k = 0; k < p->units.size(); ++k) {
+        const size_t n = unit_elems(ND, p, k);
+        K.q.push_back((signed char*)A.take((n + 3) / 4));
+        K.scale.push_back(A.take((n + 63) / 64));
+        K.vec.push_back(A.take(vec_floats(p->units[k].cout)));
+    }
+    K.bytes = A.off;
+}
+// what both directions check and lay out
+int kept8_open(const e3_unet_plan* plan, int N, int D, int H, int W, void* saved, size_t saved_bytes, void* kept, size_t kept_bytes, NetDims& ND, Buffers& B, Kept8& K) {
+    E3_REQUIRE(plan && N > 0 && D > 0 && H > 0 && W > 0 && saved && kept, E3_ERR_INVALID, "bad argument");
+    E3_REQUIRE(checkpoint8_covered(plan), E3_ERR_UNSUPPORTED, "8-bit activation checkpoints: 'same' convs, transposed convs and a norm behind every conv, no attention");
+    net_dims(plan, N, D, H, W, ND);
+    E3_REQUIRE(ND.ok, E3_ERR_INVALID, "input too small for this network");
+    plan_buffers(plan, N, D, H, W, true, saved, nullptr, B);
+    E3_REQUIRE(saved_bytes >= B.saved_bytes, E3_ERR_WORKSPACE, "`saved` buffer too small");
+    kept8_layout(plan, ND, kept, K);
+    E3_REQUIRE(kept_bytes >= K.bytes, E3_ERR_WORKSPACE, "`kept` buffer too small");
+    return E3_OK;
+}
+}  // namespace
+
+int e3_unet_checkpoint8_bytes(const e3_unet_plan* plan, int N, int D, int H, int W, size_t* kept_bytes) {
+    E3_REQUIRE(plan && N > 0 && D > 0 && H > 0 && W > 0 && kept_bytes, E3_ERR_INVALID, "bad argument");
+    E3_REQUIRE(checkpoint8_covered(plan), E3_ERR_UNSUPPORTED, "8-bit activation checkpoints: 'same' convs, transposed convs and a norm behind every conv, no attention");
+    NetDims ND; net_dims(plan, N, D, H, W, ND);
+    E3_REQUIRE(ND.ok, E3_ERR_INVALID, "input too small for this network");
+    Kept8 K; kept8_layout(plan, ND, nullptr, K);
+    *kept_bytes = K.bytes;
+    return E3_OK;
+}
+
+int e3_unet_checkpoint8_keep(const e3_unet_plan* plan, void* stream, int N, int D, int H, int W, const void* saved, size_t saved_bytes, void* kept, size_t kept_bytes) {
+    NetDims ND; Buffers B; Kept8 K;
+    RUN(kept8_open(plan, N, D, H, W, const_cast<void*>(saved), saved_bytes, kept, kept_bytes, ND, B, K));
+    hipStream_t s = (hipStream_t)stream;
+    std::vector<CopyJob> copies;
+    for (size_t k = 0; k < plan->units.size(); ++k) {
+        const int C = plan->units[k].cout;
+        RUN(launch_checkpoint8_pack(E3_DT_F32, B.ub[k].raw, C, (long long)ND.u[k].out.vox, C, K.q[k], K.scale[k], s));
+        copies.push_back({B.ub[k].mean, K.vec[k], vec_floats(C)});
+    }
+    if (K.xin_floats) copies.push_back({B.xin, K.xin, K.xin_floats});
+    return launch_copy_multi(copies.data(), (int)copies.size(), s);
+}
+
+int e3_unet_checkpoint8_restore(const e3_unet_plan* plan, void* stream, int N, int D, int H, int W, void* const* params, const void* kept, size_t kept_bytes,
+                                void* saved, size_t saved_bytes) {
+    E3_REQUIRE(params, E3_ERR_INVALID, "null argument");
+    NetDims ND; Buffers B; Kept8 K;
+    RUN(kept8_open(plan, N, D, H, W, saved, saved_bytes, const_cast<void*>(kept), kept_bytes, ND, B, K));
+    hipStream_t s = (hipStream_t)stream;
+    std::vector<CopyJob> copies;
+    for (size_t k = 0; k < plan->units.size(); ++k) copies.push_back({K.vec[k], B.ub[k].mean, vec_floats(plan->units[k].cout)});
+    if (K.xin_floats) copies.push_back({K.xin, B.xin, K.xin_floats});
+    RUN(launch_copy_multi(copies.data(), (int)copies.size(), s));
+    const int nb = plan->cfg.n_blocks;
+    for (size_t k = 0; k < plan->units.size(); ++k) {
+        const ConvUnit& u = plan->units[k];
+        const UnitBufs& b = B.ub[k];
+        const LevelDims& lo = ND.u[k].out;
+        RUN(launch_checkpoint8_unpack(E3_DT_F32, K.q[k], K.scale[k], (long long)lo.vox, u.cout, b.raw, u.cout, s));
+        if (k + 1 == plan->units.size()) break;        // (the head reads the raw tensor)
+        const ActArg act = plan->rrelu_of(u.p_a >= 0 ? ActArg(0.f, (const float*)params[u.p_a]) : ActArg(plan->cfg.act_slope), (int)k);
+        RUN(launch_bn_relu_apply(b.raw, u.cout, b.scale, b.shift, b.act, b.act_ldc, u.enc_last && u.level < nb - 1 ? B.pooled[u.level] : nullptr, u.planar ? 1 : 2,
+                                 N, lo.D, lo.H, lo.W, u.cout, s, act));
+        if (u.is_up && plan->cfg.merge_add)
+            RUN(launch_add_views(B.cat[u.level], 2 * u.cout, B.cat[u.level] + u.cout, 2 * u.cout, B.sum[u.level], u.cout, lo.vox, u.cout, s));
+    }
     return E3_OK;
 }
 

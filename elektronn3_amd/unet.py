@@ -133,6 +133,30 @@ def _alloc_saved(device, nbytes):
     return torch.empty(int(nbytes), dtype=torch.uint8, device=device)
 
 
+class _Kept8:
+    """The `saved` arena of a training forward in 8 bits (e3_unet_checkpoint8_keep / _restore): what the autograd node holds with ``UNet.checkpoint8()``."""
+    __slots__ = ('plan', 'dims', 'buf', 'nbytes')
+
+    def __init__(self, plan, dims, saved):
+        lib = _lib.load()
+        n = c_size_t()
+        check(lib.e3_unet_checkpoint8_bytes(plan.handle, *dims, ctypes.byref(n)))
+        self.plan, self.dims, self.nbytes = plan, dims, saved.numel()
+        self.buf = torch.empty(n.value, dtype=torch.uint8, device=saved.device)
+        with torch.cuda.device(saved.device):
+            check(lib.e3_unet_checkpoint8_keep(plan.handle, _lib.stream_ptr(saved.device), *dims, c_void_p(saved.data_ptr()), c_size_t(saved.numel()),
+                                               c_void_p(self.buf.data_ptr()), c_size_t(self.buf.numel())))
+
+    def restore(self, tens):
+        dev = self.buf.device
+        saved = _alloc_saved(dev, self.nbytes)
+        ptrs = (c_void_p * len(tens))(*[t.data_ptr() for t in tens])
+        with torch.cuda.device(dev):
+            check(_lib.load().e3_unet_checkpoint8_restore(self.plan.handle, _lib.stream_ptr(dev), *self.dims, ptrs, c_void_p(self.buf.data_ptr()), c_size_t(self.buf.numel()),
+                                                          c_void_p(saved.data_ptr()), c_size_t(saved.numel())))
+        return saved
+
+
 def release_scratch():
     """Drop the cached scratch buffers (they are re-created on the next call)."""
     _scratch.clear()
@@ -177,7 +201,7 @@ def _fp32_table(module, tens):
     return cache[2]
 
 
-def _native_forward(module, plan, x, tens, softmax, want16, x_needs_grad, training, momenta, frozen=False, loss=None, roi=None):
+def _native_forward(module, plan, x, tens, softmax, want16, x_needs_grad, training, momenta, frozen=False, loss=None, roi=None, keep8=False):
     """One call of e3_unet_forward / e3_unet_forward_bf16 / e3_unet_forward_f16.  `tens`: fp32 table tensors (contiguous); `want16`: None, or
     the 16-bit type to compute in (torch.bfloat16 / torch.float16).  Returns (y fp32, saved buffer or None, the input as handed to the
     library, the 16-bit type of the native path taken or None)."""
@@ -185,6 +209,8 @@ def _native_forward(module, plan, x, tens, softmax, want16, x_needs_grad, traini
     dev = x.device
     N, Cin, D, H, W = x.shape
     b16 = want16 if (want16 and not x_needs_grad and not frozen and plan.bf16_supported() and not _NO_BF16) else None
+    if keep8 and b16 is not None:
+        raise NotImplementedError('checkpoint8: the 16-bit kernels keep their activations as they are (fp32 compute only)')
     xin = x.detach().to(b16 if b16 is not None else torch.float32).contiguous()
     saved_bytes, scratch_bytes = plan.sizes(N, D, H, W, training, bf16=b16)
     saved = _alloc_saved(dev, max(saved_bytes, 256)) if training else None
@@ -407,7 +433,7 @@ class _UNetFunction(torch.autograd.Function):
                                              ctx.needs_input_grad[3], training or frozen,
                                              module._momenta(plan) if (training or frozen) else None, frozen=frozen,
                                              loss=loss_req if (training and not softmax) else None,
-                                             roi=roi if not (training or frozen) else None)
+                                             roi=roi if not (training or frozen) else None, keep8=need_grad and bool(module.__dict__.get('_checkpoint8')))
         if getattr(module, 'attention', False) and b16 is None:
             _store_attention_maps(module, plan, x, training or frozen, saved)
         ctx.frozen = frozen
@@ -424,6 +450,8 @@ class _UNetFunction(torch.autograd.Function):
         ctx.softmax, ctx.eval_mode, ctx.in_dtype = softmax, not (training or frozen), in_dtype
         # (a low-precision module's fp32 table is a cache that the next forward refreshes with the same parameter values:
         # the backward only reads weights and affine parameters from it, never the running statistics)
+        if need_grad and module.__dict__.get('_checkpoint8'):
+            saved = _Kept8(plan, (xin.shape[0], *xin.shape[2:]), saved)
         ctx.x32, ctx.saved_buf, ctx.tens = (xin, saved, _TableRef(tens, False)) if need_grad else (None, None, None)
         if need_grad and lowp is not None:
             # the fp32 table of a low-precision module is ONE persistent cache that the next forward overwrites in place: this forward registers its
@@ -444,7 +472,8 @@ class _UNetFunction(torch.autograd.Function):
             raise NotImplementedError('backward through the fused softmax head is not implemented')
         module, plan = ctx.module, ctx.plan
         check(_lib.load().e3_unet_set_rrelu(plan.handle, *(ctx.rrelu if ctx.rrelu is not None else (0.0, 0.0, 0))))
-        flat, views, dx = _native_backward(plan, dy, ctx.x32, ctx.tens.tens, ctx.saved_buf, ctx.b16, ctx.needs_input_grad[3],
+        saved = ctx.saved_buf.restore(ctx.tens.tens) if isinstance(ctx.saved_buf, _Kept8) else ctx.saved_buf
+        flat, views, dx = _native_backward(plan, dy, ctx.x32, ctx.tens.tens, saved, ctx.b16, ctx.needs_input_grad[3],
                                            getattr(module, '_grad_sync', None), frozen=ctx.frozen, loss=getattr(ctx, 'loss_bwd', None))
         ctx.loss_bwd = None
         ctx.saved_buf = ctx.x32 = ctx.tens = None   # free the activations now
@@ -1235,9 +1264,25 @@ class UNet(nn.Module):
             _packed_ok(pkey, token)
 
     @torch.jit.unused
+    def checkpoint8(self, enabled=True):
+        """Keeps the activations of training forwards in 8 bits until their backward (about 1/7 of the memory of a pending graph; the forward and the backward
+        each need the full buffer while they run).  For several graphs that are alive at once: accumulation over networks or views, and
+        ``normalization='group'`` / ``'instance'``, whose batch is one graph per sample.  The outputs are unchanged; the gradients are those of the rounded
+        tensors: of every norm's input, an element is off by at most 1/254 of the largest of its block of 64 (:class:`elektronn3_amd.ops.Checkpoint8`),
+        and the activations are recomputed from them.  What the reference's ``forward_gradcp`` (unet.py:918-935) trades recomputation for, this trades
+        precision for.  fp32 compute; transposed up-convolutions, 'same' convolutions and a norm behind every convolution, no attention
+        (NotImplementedError otherwise).  Scripted modules keep their activations as they are.  Returns the module."""
+        if enabled:
+            n = c_size_t()
+            size = 2 ** self.n_blocks
+            check(_lib.load().e3_unet_checkpoint8_bytes(self._plan().handle, 1, 1 if self.dim == 2 else size, size, size, ctypes.byref(n)))
+        self.__dict__['_checkpoint8'] = bool(enabled)
+        return self
+
+    @torch.jit.unused
     def forward_gradcp(self, x):
         """Same as :meth:`forward` (unet.py:918-935 trades recompute for memory; with 288 GB of HBM nothing needs to be
-        recomputed, so checkpointing is a no-op here)."""
+        recomputed, so checkpointing is a no-op here; see :meth:`checkpoint8` for less memory per pending graph)."""
         return self.forward(x)
 
     # profiling hook used by bench.py (roofline of a single layer measured with HIP events inside the step)

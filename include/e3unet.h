@@ -185,6 +185,18 @@ int e3_unet_backward_loss(e3_unet_plan* plan, void* stream, const float* y, cons
                           void* saved, size_t saved_bytes, void* scratch, size_t scratch_bytes,
                           void* bucket_event, int bucket_after_down_block, uint32_t flags);
 
+/* The activations that a training forward left in `saved`, kept in 8 bits until the backward (what UNet.forward_gradcp trades recomputation
+ * for, unet.py:918-935): _keep writes the raw conv outputs of `saved` as 8-bit checkpoints (see e3_checkpoint8_pack) beside the norms' fp32
+ * vectors into `kept` (e3_unet_checkpoint8_bytes() bytes, about 1/7 of `saved`), after which `saved` may be reused; _restore fills a `saved`
+ * buffer for e3_unet_backward* of the same plan, shape and parameters, recomputing the activations from the restored tensors (the gradients are
+ * those of the rounded tensors).  nn.RReLU: e3_unet_set_rrelu with the forward's seed first.  fp32 path; 'same' convs, transposed convs and a
+ * norm behind every conv, no attention, not the ResUNet (E3_ERR_UNSUPPORTED otherwise). */
+int e3_unet_checkpoint8_bytes(const e3_unet_plan* plan, int N, int D, int H, int W, size_t* kept_bytes);
+int e3_unet_checkpoint8_keep(const e3_unet_plan* plan, void* stream, int N, int D, int H, int W, const void* saved, size_t saved_bytes,
+                             void* kept, size_t kept_bytes);
+int e3_unet_checkpoint8_restore(const e3_unet_plan* plan, void* stream, int N, int D, int H, int W, void* const* params,
+                                const void* kept, size_t kept_bytes, void* saved, size_t saved_bytes);
+
 /* Per-layer profiling hook used by bench.py for the roofline line: when `layer` >= 0, hipEvents are recorded
  * around that layer's dominant kernel in every subsequent forward (which=0), dgrad (1) or wgrad (2); read the
  * mean duration of all recorded launches (and reset) with e3_unet_profile_read.  `layer` indexes the conv list
