@@ -6,6 +6,10 @@
 // stay zero (a ReLU's border); 64 elements, because a block is then 8 lanes of 8 elements (16-byte pieces of a 16-bit tensor) and the scales cost 1/16 of the
 // codes.  The step is amax / 127, the error of an element at most half of it.  amax < 2^-110: the block is kept as zeros (scale 0; 127 / amax would
 // overflow).  A block that holds a NaN or an infinity gets scale NaN: all of it comes back as NaN, so that a diverged activation stays visible.
+//
+// A checkpoint of the input of a norm with ReLU / LeakyReLU is rounded TO ITS SIDE: where x and its rounded value lie on different sides of the activation's border
+// (z = 0), the code is the other neighbour of x, which lies on x's side.  The error there is up to a whole step, but the backward then takes exactly the forward's
+// branch everywhere.  Rounded to nearest, 1 element in 400 of a Gaussian changes sides, and each contributes its whole gradient: 7 % of a layer's gradient norm.
 #pragma once
 #include "common.h"
 
@@ -118,6 +122,17 @@ template <int V> __device__ __forceinline__ Codes<V> encode_block(const float (&
     for (int e = 0; e < V; ++e) c.q[e] = (none || bad) ? (signed char)0 : (signed char)(int)rintf(f[e] * inv);
     return c;
 }
+// the value of code e
+template <int V> __device__ __forceinline__ float code_value(const Codes<V>& c, int e) {
+#pragma clang fp contract(off)
+    return (float)c.q[e] * c.scale;
+}
+// code q of x with value v, moved to the other neighbour of x
+__device__ __forceinline__ signed char other_neighbour(signed char q, float x, float v) {
+    const int m = (int)q + (x > v ? 1 : -1);
+    return (signed char)(m > 127 ? 127 : m < -127 ? -127 : m);
+}
+
 template <int V> __device__ __forceinline__ void store_codes(const Codes<V>& c, signed char* q, float* scale, size_t e) {
     if constexpr (V == 1) q[e] = c.q[0];
     else {
@@ -138,6 +153,10 @@ inline bool wide_codes(int dt, const void* q, int C) { return C % wide_of(dt) ==
 
 }  // namespace e3n
 
-// (stream, type, view of x, its checkpoint): launchers shared with the fused forms
-int launch_checkpoint8_pack(int dt, const void* x, int x_ldc, long long vox, int C, signed char* q, float* scale, hipStream_t s);
+// Which side of the border an element is on, for the pass that writes a checkpoint by itself.  rule 0: no border; 1: the exact sign of (x - mean) rstd gamma + beta
+// with mean, rstd [N][G] and gamma, beta [C] or nullptr (what group_norm.hip decides by), S voxels to a sample; 2: the sign of fmaf(x, a[c], b[c]) (elementwise.hip)
+struct Border { int rule = 0; const float *mean = nullptr, *rstd = nullptr, *gamma = nullptr, *beta = nullptr; const float *a = nullptr, *b = nullptr; long long S = 1; int G = 1; };
+
+// launchers shared with the fused forms
+int launch_checkpoint8_pack(int dt, const void* x, int x_ldc, long long vox, int C, signed char* q, float* scale, const Border& border, hipStream_t s);
 int launch_checkpoint8_unpack(int dt, const signed char* q, const float* scale, long long vox, int C, void* y, int y_ldc, hipStream_t s);

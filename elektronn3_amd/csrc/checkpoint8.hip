@@ -22,9 +22,17 @@ template <int V, bool DENSE> __device__ __forceinline__ size_t piece_offset(size
     }
 }
 
-template <int DT, int V, bool DENSE, bool NT>
+__device__ __forceinline__ bool positive(const Border& d, float x, size_t e, int C) {
+    const size_t v = e < 0xffffffffu ? (size_t)((unsigned)e / (unsigned)C) : e / (size_t)C;
+    const int c = (int)(e - v * (size_t)C);
+    if (d.rule == 2) return __builtin_fmaf(x, d.a[c], d.b[c]) > 0.f;
+    const size_t g = (v / (size_t)d.S) * d.G + c / (C / d.G);
+    return ((double)x - (double)d.mean[g]) * (double)d.rstd[g] * (d.gamma ? (double)d.gamma[c] : 1.0) + (d.beta ? (double)d.beta[c] : 0.0) > 0.0;
+}
+
+template <int DT, int V, bool DENSE, bool NT, bool SIDE>
 __global__ __launch_bounds__(BT) void checkpoint8_pack_kernel(const typename Elem<DT>::T* __restrict__ x, int ldc, int C, size_t n,
-                                                              signed char* __restrict__ q, float* __restrict__ scale) {
+                                                              signed char* __restrict__ q, float* __restrict__ scale, const Border border) {
     constexpr int U = DT == DT_F32 ? 8 : 4;                  // pieces in flight per lane
     const size_t step = (size_t)gridDim.x * BT * V;
     // (the loop's condition is the workgroup's: every lane of a wave reaches the reduction inside encode_block)
@@ -41,8 +49,17 @@ __global__ __launch_bounds__(BT) void checkpoint8_pack_kernel(const typename Ele
         for (int u = 0; u < U; ++u) {
             float f[V];
             unpack_raw<DT, V>(raw[u], f);
-            const Codes<V> c = encode_block<V>(f);
-            if (ok[u]) store_codes<V>(c, q, scale, b0 + u * step + (size_t)threadIdx.x * V);
+            Codes<V> c = encode_block<V>(f);
+            const size_t e0 = b0 + u * step + (size_t)threadIdx.x * V;
+            if constexpr (SIDE) {
+                if (ok[u] && c.scale > 0.f)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        const float v = code_value<V>(c, e);
+                        if (positive(border, f[e], e0 + e, C) != positive(border, v, e0 + e, C)) c.q[e] = other_neighbour(c.q[e], f[e], v);
+                    }
+            }
+            if (ok[u]) store_codes<V>(c, q, scale, e0);
         }
     }
 }
@@ -72,11 +89,11 @@ unsigned grid_for(size_t n, int V) {
     return (unsigned)(blocks < 2048 ? blocks : 2048);       // 8 workgroups of 4 waves per CU, grid-stride beyond
 }
 
-template <int DT, int V, bool NT>
-void pack_nt(const void* x, int ldc, size_t n, int C, signed char* q, float* scale, hipStream_t s) {
+template <int DT, int V, bool NT, bool SIDE>
+void pack_nt(const void* x, int ldc, size_t n, int C, signed char* q, float* scale, const Border& b, hipStream_t s) {
     typedef const typename Elem<DT>::T* P;
-    if (ldc == C) hipLaunchKernelGGL((checkpoint8_pack_kernel<DT, V, true, NT>), dim3(grid_for(n, V)), dim3(BT), 0, s, (P)x, ldc, C, n, q, scale);
-    else hipLaunchKernelGGL((checkpoint8_pack_kernel<DT, V, false, NT>), dim3(grid_for(n, V)), dim3(BT), 0, s, (P)x, ldc, C, n, q, scale);
+    if (ldc == C) hipLaunchKernelGGL((checkpoint8_pack_kernel<DT, V, true, NT, SIDE>), dim3(grid_for(n, V)), dim3(BT), 0, s, (P)x, ldc, C, n, q, scale, b);
+    else hipLaunchKernelGGL((checkpoint8_pack_kernel<DT, V, false, NT, SIDE>), dim3(grid_for(n, V)), dim3(BT), 0, s, (P)x, ldc, C, n, q, scale, b);
 }
 template <int DT, int V, bool NT>
 void unpack_nt(const signed char* q, const float* scale, size_t n, int C, void* y, int ldc, hipStream_t s) {
@@ -85,9 +102,10 @@ void unpack_nt(const signed char* q, const float* scale, size_t n, int C, void* 
     else hipLaunchKernelGGL((checkpoint8_unpack_kernel<DT, V, false, NT>), dim3(grid_for(n, V)), dim3(BT), 0, s, q, scale, n, C, ldc, (P)y);
 }
 template <int DT, int V>
-void pack_typed(const void* x, int ldc, size_t n, int C, signed char* q, float* scale, hipStream_t s) {
-    if (V > 1 && n * sizeof(typename Elem<DT>::T) >= CACHE_BYTES) pack_nt<DT, V, (V > 1)>(x, ldc, n, C, q, scale, s);
-    else pack_nt<DT, V, false>(x, ldc, n, C, q, scale, s);
+void pack_typed(const void* x, int ldc, size_t n, int C, signed char* q, float* scale, const Border& b, hipStream_t s) {
+    if (b.rule) pack_nt<DT, V, false, true>(x, ldc, n, C, q, scale, b, s);
+    else if (V > 1 && n * sizeof(typename Elem<DT>::T) >= CACHE_BYTES) pack_nt<DT, V, (V > 1), false>(x, ldc, n, C, q, scale, b, s);
+    else pack_nt<DT, V, false, false>(x, ldc, n, C, q, scale, b, s);
 }
 template <int DT, int V>
 void unpack_typed(const signed char* q, const float* scale, size_t n, int C, void* y, int ldc, hipStream_t s) {
@@ -102,16 +120,16 @@ bool wide(int dt, const void* p, int ldc, int C, size_t n, const void* q) {
 
 }  // namespace
 
-int launch_checkpoint8_pack(int dt, const void* x, int x_ldc, long long vox, int C, signed char* q, float* scale, hipStream_t s) {
+int launch_checkpoint8_pack(int dt, const void* x, int x_ldc, long long vox, int C, signed char* q, float* scale, const Border& border, hipStream_t s) {
     const size_t n = (size_t)vox * C;
     if (n == 0) return E3_OK;
     switch (dt * 2 + wide(dt, x, x_ldc, C, n, q)) {
-        case 0: pack_typed<DT_F32, 1>(x, x_ldc, n, C, q, scale, s); break;
-        case 1: pack_typed<DT_F32, 4>(x, x_ldc, n, C, q, scale, s); break;
-        case 2: pack_typed<DT_BF16, 1>(x, x_ldc, n, C, q, scale, s); break;
-        case 3: pack_typed<DT_BF16, 8>(x, x_ldc, n, C, q, scale, s); break;
-        case 4: pack_typed<DT_F16, 1>(x, x_ldc, n, C, q, scale, s); break;
-        default: pack_typed<DT_F16, 8>(x, x_ldc, n, C, q, scale, s); break;
+        case 0: pack_typed<DT_F32, 1>(x, x_ldc, n, C, q, scale, border, s); break;
+        case 1: pack_typed<DT_F32, 4>(x, x_ldc, n, C, q, scale, border, s); break;
+        case 2: pack_typed<DT_BF16, 1>(x, x_ldc, n, C, q, scale, border, s); break;
+        case 3: pack_typed<DT_BF16, 8>(x, x_ldc, n, C, q, scale, border, s); break;
+        case 4: pack_typed<DT_F16, 1>(x, x_ldc, n, C, q, scale, border, s); break;
+        default: pack_typed<DT_F16, 8>(x, x_ldc, n, C, q, scale, border, s); break;
     }
     E3_CHECK_HIP(hipGetLastError());
     return E3_OK;
@@ -138,7 +156,7 @@ int e3_checkpoint8_pack(void* stream, int dtype, const void* x, int x_ldc, long 
     E3_REQUIRE(dtype >= 0 && dtype <= 2, E3_ERR_INVALID, "dtype must be E3_DT_F32, E3_DT_BF16 or E3_DT_F16");
     E3_REQUIRE(C >= 1 && voxels >= 0 && x_ldc >= C, E3_ERR_INVALID, "bad sizes");
     E3_REQUIRE(voxels == 0 || (x && q && scale), E3_ERR_INVALID, "null argument");
-    return launch_checkpoint8_pack(dtype, x, x_ldc, voxels, C, q, scale, (hipStream_t)stream);
+    return launch_checkpoint8_pack(dtype, x, x_ldc, voxels, C, q, scale, Border(), (hipStream_t)stream);
 }
 
 int e3_checkpoint8_unpack(void* stream, int dtype, const signed char* q, const float* scale, long long voxels, int C, void* y, int y_ldc) {

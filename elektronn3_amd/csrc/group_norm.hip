@@ -178,6 +178,45 @@ template <bool SILU> __device__ __forceinline__ float activate(float z, float sl
     else return z <= 0.f ? (slope == 0.f ? 0.f : slope * z) : z;       // NaN stays NaN
 }
 
+// |z| below which the fp32 evaluation of z may have the wrong sign: its rounding error is below 2^-21 of |(x - mean) a|, which is |beta| up to a factor 2 there
+template <int V, int UN> __device__ __forceinline__ float border_of(const Consts<V, UN>& k) {
+    float m = 0.f;
+#pragma unroll
+    for (int e = 0; e < V; ++e) m = fmaxf(m, fabsf(k.b[e]));
+    return m * 0x1p-20f;
+}
+__device__ __forceinline__ bool positive_exact(float x, float mu, float rs, double ga, double be) { return ((double)x - (double)mu) * (double)rs * ga + be > 0.0; }
+
+// The codes of a piece moved to the side of the activation's border that their elements are on (see checkpoint8.h); pieces with an element at the border itself are
+// decided again in fp64, in a rolled loop (unrolled, hipcc computes its operands in front of the voxel loop and keeps them in registers).
+template <int V, int UN>
+__device__ __forceinline__ void keep_side(const GnArgs& a, int c, const float (&x)[V], const Consts<V, UN>& k, float border, Codes<V>& q) {
+    if (!(q.scale > 0.f)) return;
+    float least = 3.4e38f, v[V];
+    unsigned moved = 0;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        v[e] = code_value<V>(q, e);
+        const float z = __builtin_fmaf(x[e] - k.mu[e / UN], k.a[e], k.b[e]), zq = __builtin_fmaf(v[e] - k.mu[e / UN], k.a[e], k.b[e]);
+        least = fminf(least, fminf(fabsf(z), fabsf(zq)));
+        moved |= ((z > 0.f) != (zq > 0.f)) ? 1u << e : 0u;
+    }
+    if (least < border) {
+        moved = 0;
+#pragma unroll 1
+        for (int e = 0; e < V; ++e) {
+            float xe = x[0], ve = v[0], mu = k.mu[0], rs = k.rs[0];
+#pragma unroll
+            for (int j = 1; j < V; ++j) { xe = e == j ? x[j] : xe; ve = e == j ? v[j] : ve; mu = e == j ? k.mu[j / UN] : mu; rs = e == j ? k.rs[j / UN] : rs; }
+            const double ga = a.gamma ? (double)a.gamma[c + e] : 1.0, be = a.beta ? (double)a.beta[c + e] : 0.0;
+            moved |= positive_exact(xe, mu, rs, ga, be) != positive_exact(ve, mu, rs, ga, be) ? 1u << e : 0u;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+        if (moved >> e & 1) q.q[e] = other_neighbour(q.q[e], x[e], v[e]);
+}
+
 // ------------------------------------------------------------------------------------------------ forward
 // Sums and sums of squares in fp64: the variance is then a difference that loses nothing an fp32 input holds, whatever its mean.
 template <int V, int UN> struct Moments {
@@ -255,7 +294,8 @@ __global__ __launch_bounds__(MAX_T) void gn_apply_kernel(const GnArgs a) {
     }
     Consts<V, UN> k{};
     if (w.on) k = constants<V, UN>(a, mean, rstd, w.c);
-    // (KEEP: every lane goes round together -- the checkpoint's blocks are 8 lanes)
+    const float border = border_of<V, UN>(k);
+    // (KEEP: every lane goes round together -- a checkpoint's block is 8 or 16 lanes)
     for (;;) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -263,7 +303,8 @@ __global__ __launch_bounds__(MAX_T) void gn_apply_kernel(const GnArgs a) {
             in[u].get(f);
             const size_t row = (size_t)(w.n * a.S + vb + w.r + u * a.R);
             if constexpr (KEEP) {
-                const Codes<V> c = encode_block<V>(f);
+                Codes<V> c = encode_block<V>(f);
+                if constexpr (!SILU) if (ok[u] && a.slope != 1.f) keep_side<V, UN>(a, w.c, f, k, border, c);
                 if (ok[u]) store_codes<V>(c, a.q_out, a.qs_out, row * a.C + w.c);
             }
 #pragma unroll
@@ -323,12 +364,13 @@ __global__ __launch_bounds__(MAX_T) void gn_fwd_group_kernel(const GnArgs a) {
         in[k].get(f);
         const size_t row = (size_t)(n * a.S + v);
         if constexpr (KEEP) {                // (bundles of whole blocks)
-            const Codes<V> q = encode_block<V>(f);
+            Codes<V> q = encode_block<V>(f);
+            if constexpr (!SILU) if (ok && a.slope != 1.f) keep_side<V, UN>(a, c, f, k0, border_of<V, UN>(k0), q);
             if (ok) store_codes<V>(q, a.q_out, a.qs_out, row * a.C + c);
         }
 #pragma unroll
         for (int e = 0; e < V; ++e) o[e] = activate<SILU>(__builtin_fmaf(f[e] - k0.mu[e / UN], k0.a[e], k0.b[e]), a.slope);
-        if (ok) store_f32<DT, V>((T*)a.out + row * a.out_ldc + c, o);
+        if (ok && a.out) store_f32<DT, V>((T*)a.out + row * a.out_ldc + c, o);      // (no output: the statistics alone)
     }
 }
 
@@ -361,7 +403,7 @@ __device__ __forceinline__ void grad_piece(const GnArgs& a, int n, int c, const 
                 float xe = x[0], ge = g[0];
 #pragma unroll
                 for (int j = 1; j < V; ++j) { xe = e == j ? x[j] : xe; ge = e == j ? g[j] : ge; }
-                const bool pos = ((double)xe - (double)a.mean[i]) * (double)a.rstd[i] * ga + be > 0.0;
+                const bool pos = positive_exact(xe, a.mean[i], a.rstd[i], ga, be);
                 const float d = pos ? ge : (a.slope == 0.f ? 0.f : a.slope * ge);
 #pragma unroll
                 for (int j = 0; j < V; ++j) dz[j] = e == j ? d : dz[j];
@@ -369,13 +411,6 @@ __device__ __forceinline__ void grad_piece(const GnArgs& a, int n, int c, const 
         }
     }
 }
-template <int V, int UN> __device__ __forceinline__ float border_of(const Consts<V, UN>& k) {
-    float m = 0.f;
-#pragma unroll
-    for (int e = 0; e < V; ++e) m = fmaxf(m, fabsf(k.b[e]));
-    return m * 0x1p-20f;
-}
-
 // Per-thread sums of dz and dz t (h = t rstd: the factor comes last) in fp32 over at most a chunk's voxels / R, everything behind them in fp64.
 template <int DT, int V, int UN, bool CK, bool SILU>
 __global__ __launch_bounds__(MAX_T) void gn_bwd_reduce_kernel(const GnArgs a) {
@@ -615,6 +650,13 @@ template <int DT, int V, int UN, bool CK, bool BEHIND> void launch_apply(GnArgs 
     GN_LAUNCH((gn_apply_kernel<DT, V, UN, CK, SILU, false, NT>), grid_of(a), block_of(a), lds, s, a);
 }
 
+// the checkpoint as a pass of its own, behind the one that has written mean and rstd
+int pack_behind(int dt, const GnArgs& a, const Shape& sh, hipStream_t s) {
+    Border b;
+    if (a.slope != 1.f && a.slope != ACT_SILU) { b.rule = 1; b.mean = a.mean_out; b.rstd = a.rstd_out; b.gamma = a.gamma; b.beta = a.beta; b.S = sh.S; b.G = sh.G; }
+    return launch_checkpoint8_pack(dt, a.x, a.x_ldc, (long long)sh.N * sh.S, sh.C, a.q_out, a.qs_out, b, s);
+}
+
 template <int DT, int V, int UN> int forward_group(GnArgs a, const Shape& sh, hipStream_t s) {
     const dim3 grid((unsigned)((long long)sh.N * (a.P / a.PT)));
     if constexpr (V > 1 && UN == V) {
@@ -623,9 +665,16 @@ template <int DT, int V, int UN> int forward_group(GnArgs a, const Shape& sh, hi
             return E3_OK;
         }
     }
-    if (a.q_out) { const int rc = launch_checkpoint8_pack(DT, a.x, a.x_ldc, (long long)sh.N * sh.S, sh.C, a.q_out, a.qs_out, s); if (rc) return rc; }
+    if (a.q_out && a.out == a.x) {           // in place: the checkpoint, which needs the statistics, in front of the output
+        GnArgs st = a;
+        st.out = nullptr;
+        GN_LAUNCH((gn_fwd_group_kernel<DT, V, UN, SILU, false>), grid, block_of(a), 0, s, st);
+        const int rc = pack_behind(DT, a, sh, s);
+        if (rc) return rc;
+        a.q_out = nullptr;
+    }
     GN_LAUNCH((gn_fwd_group_kernel<DT, V, UN, SILU, false>), grid, block_of(a), 0, s, a);
-    return E3_OK;
+    return a.q_out ? pack_behind(DT, a, sh, s) : E3_OK;
 }
 
 template <int DT, int V, int UN> int forward(GnArgs a, const Shape& sh, void* ws, hipStream_t s) {
@@ -640,19 +689,18 @@ template <int DT, int V, int UN> int forward(GnArgs a, const Shape& sh, void* ws
     const int units = sh.C / UN, per = st.cg / UN;
     hipLaunchKernelGGL((gn_stats_kernel<DT, V, UN>), grid_of(st), block_of(st), (size_t)st.R * st.PT * (V / UN) * 2 * sizeof(double), s, st);
     a.mean = a.mean_out; a.rstd = a.rstd_out;
-    if ((long long)st.chunks * units <= MERGE_MAX && units <= MERGE_UNITS) { a.rec = st.part; a.rec_chunks = st.chunks; a.rec_units = units; a.rec_per = per; }
-    else hipLaunchKernelGGL(gn_finalize_kernel, dim3(sh.N * sh.G), dim3(256), 0, s, st.part, st.chunks, units, per, st.inv_m, a.eps, a.mean_out, a.rstd_out);
-    // the checkpoint rides in the apply pass where its blocks are whole there; otherwise it is a pass of its own
+    // the checkpoint rides in the apply pass where its blocks are whole there; otherwise it is a pass of its own: behind the apply pass, or, in place, in front of it
     GnArgs m{}; map_pass<V>(m, sh, PASS_WGS, U1<V>, true);
     const bool fused = a.q_out && V > 1 && m.tiles == 1 && m.R * m.PT <= MAX_T && ((unsigned long long)sh.S * sh.C) % CK_BLOCK == 0 && (uintptr_t)a.q_out % V == 0;
-    if (a.q_out && !fused) {
-        const int rc = launch_checkpoint8_pack(DT, a.x, a.x_ldc, (long long)sh.N * sh.S, sh.C, a.q_out, a.qs_out, s);
-        if (rc) return rc;
-        a.q_out = nullptr;
-    }
-    launch_apply<DT, V, UN, false, true>(a, sh, s);
+    const bool before = a.q_out && !fused && a.out == a.x;
+    if (!before && (long long)st.chunks * units <= MERGE_MAX && units <= MERGE_UNITS) { a.rec = st.part; a.rec_chunks = st.chunks; a.rec_units = units; a.rec_per = per; }
+    else hipLaunchKernelGGL(gn_finalize_kernel, dim3(sh.N * sh.G), dim3(256), 0, s, st.part, st.chunks, units, per, st.inv_m, a.eps, a.mean_out, a.rstd_out);
+    if (before) { const int rc = pack_behind(DT, a, sh, s); if (rc) return rc; }
+    GnArgs ap = a;
+    if (!fused) ap.q_out = nullptr;
+    launch_apply<DT, V, UN, false, true>(ap, sh, s);
     E3_CHECK_HIP(hipGetLastError());
-    return E3_OK;
+    return a.q_out && !fused && !before ? pack_behind(DT, a, sh, s) : E3_OK;
 }
 
 template <int DT, int V, int UN, bool CK> int backward(GnArgs a, const Shape& sh, void* ws, hipStream_t s) {

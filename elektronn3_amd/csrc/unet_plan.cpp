@@ -732,7 +732,9 @@ int e3_unet_checkpoint8_keep(const e3_unet_plan* plan, void* stream, int N, int 
     std::vector<CopyJob> copies;
     for (size_t k = 0; k < plan->units.size(); ++k) {
         const int C = plan->units[k].cout;
-        RUN(launch_checkpoint8_pack(E3_DT_F32, B.ub[k].raw, C, (long long)ND.u[k].out.vox, C, K.q[k], K.scale[k], s));
+        Border side;          // (the rounded tensors take the forward's branch of every ReLU)
+        if (plan->cfg.act_slope != 1.f && plan->cfg.act_slope != ACT_SILU) { side.rule = 2; side.a = B.ub[k].scale; side.b = B.ub[k].shift; }
+        RUN(launch_checkpoint8_pack(E3_DT_F32, B.ub[k].raw, C, (long long)ND.u[k].out.vox, C, K.q[k], K.scale[k], side, s));
         copies.push_back({B.ub[k].mean, K.vec[k], vec_floats(C)});
     }
     if (K.xin_floats) copies.push_back({B.xin, K.xin, K.xin_floats});

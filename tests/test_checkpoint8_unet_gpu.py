@@ -14,16 +14,22 @@ pytestmark = pytest.mark.gpu
 TOL = 2e-3
 
 
-def kept(x):
-    """What the 8-bit checkpoint of an NCDHW tensor stands for (blocks of 64 of the NDHWC order)."""
+def kept(x, z, border):
+    """What the 8-bit checkpoint of an NCDHW tensor stands for (blocks of 64 of the NDHWC order); border: rounded to the side of z = 0 that an element is on."""
     v = x.detach().float().movedim(1, -1).contiguous()
     flat = v.reshape(-1).numpy()
     p = np.zeros(-(-flat.size // 64) * 64, np.float32); p[:flat.size] = flat
     p = p.reshape(-1, 64)
     amax = np.abs(p).max(1, keepdims=True)
     q = np.rint(p * (np.float32(127) / np.maximum(amax, np.float32(1e-30))))
-    val = (q * (amax * np.float32(1 / 127))).reshape(-1)[:flat.size].reshape(v.shape)
-    return torch.from_numpy(val).double().movedim(-1, 1)
+    back = lambda q: torch.from_numpy((q * (amax * np.float32(1 / 127))).reshape(-1)[:flat.size].reshape(v.shape)).double().movedim(-1, 1)    # noqa: E731
+    val = back(q)
+    if border:
+        move = torch.where((z(x) > 0) != (z(val) > 0), torch.where(x > val, 1.0, -1.0), 0.0).movedim(1, -1).reshape(-1).numpy()
+        p[:] = 0
+        p.reshape(-1)[:flat.size] = move
+        val = back(np.clip(q + p, -127, 127))
+    return val
 
 
 class Norm(torch.autograd.Function):
@@ -62,7 +68,6 @@ def emulate(m, x, dy, act, groups=None, add=False, replace=True, frozen=False):
         f = (lambda t: F.conv_transpose3d(t, w, b, stride=k)) if up else (lambda t: F.conv3d(t, w, b, padding=tuple(n // 2 for n in k)))
         raw = f(a_exact).detach()
         y = f(a)
-        y = y + ((kept(raw) if replace else raw) - y).detach()
         G = raw.shape[1] if groups == 0 else groups
         if frozen:
             mean, var = (bufs[f'{norm}.running_{s}'].view(1, -1, 1, 1, 1) for s in ('mean', 'var'))
@@ -73,11 +78,13 @@ def emulate(m, x, dy, act, groups=None, add=False, replace=True, frozen=False):
             mean, var = (t.repeat_interleave(raw.shape[1] // G, 1).view(raw.shape[0], -1, 1, 1, 1) for t in (r.mean(2), r.var(2, unbiased=False)))
         inv = 1 / (var + 1e-5).sqrt()
         ga, be = (sd[f'{norm}.weight'], sd[f'{norm}.bias']) if groups != 0 else (torch.ones(raw.shape[1], dtype=torch.float64), torch.zeros(raw.shape[1], dtype=torch.float64))
+        aff = lambda t: ((t - mean) * inv * ga.view(1, -1, 1, 1, 1) + be.view(1, -1, 1, 1, 1)).detach()    # noqa: E731
+        y = y + ((kept(raw, aff, act not in ('silu', 'lin')) if replace else raw) - y).detach()
         if frozen:
             z = (y - mean) * inv * ga.view(1, -1, 1, 1, 1) + be.view(1, -1, 1, 1, 1)
         else:
             z = Norm.apply(y, ga, be, mean, inv, G)
-        ze = ((raw - mean) * inv * ga.view(1, -1, 1, 1, 1) + be.view(1, -1, 1, 1, 1)).detach()
+        ze = aff(raw)
         fn = {'relu': F.relu, 'leaky': lambda t: F.leaky_relu(t, 0.1), 'leaky2': lambda t: F.leaky_relu(t, 0.2), 'silu': F.silu, 'prelu': lambda t: F.prelu(t, sd[slope])}[act]
         return fn(z), fn(ze).detach()
 

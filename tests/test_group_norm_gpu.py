@@ -299,6 +299,19 @@ def ref_keep(x):
     return q.reshape(-1)[:n], scale, val.reshape(-1)[:n]
 
 
+def ref_side(x, q, scale, mean, rstd, w, b, act):
+    """The codes of a norm's input: where an element and its rounded value lie on different sides of a ReLU's border (64 bits), the element's other neighbour."""
+    if act in ('silu', 'lin'):
+        return q
+    C = x.shape[-1]
+    v = torch.from_numpy((q.astype(np.float64) * np.repeat(scale.astype(np.float64), 64)[:q.size]).astype(np.float32)).cuda().reshape(x.shape)
+    z = lambda t: (t.double() - spread(mean.double(), C)) * spread(rstd.double(), C) * w.double() + b.double()    # noqa: E731
+    move = (z(x) > 0) != (z(v) > 0)
+    step = torch.where(x.float() > v, 1, -1) * move
+    out = q.astype(np.int64) + step.reshape(-1).cpu().numpy()
+    return np.where(np.repeat(scale > 0, 64)[:q.size], np.clip(out, -127, 127), q).astype(np.int8)
+
+
 KEEP = [((1, 1, 1, 1, 1), None), ((1, 1, 1, 7, 9), None), ((2, 3, 5, 7, 24), None), ((2, 3, 5, 7, 24), 40), ((1, 4, 4, 4, 64), None), ((1, 2, 3, 5, 33), 50),
         ((2, 2, 9, 8, 32), 64), ((1, 1, 130, 129, 16), None), ((3, 1, 1, 1, 200), 203)]
 
@@ -350,14 +363,25 @@ def test_checkpoint_of_nothing(ops):
 @pytest.mark.parametrize('dtype', DTYPES)
 @pytest.mark.parametrize('size', SIZES)
 def test_forward_with_checkpoint_and_backward_from_it(ops, size, dtype):
-    """The checkpoint that the forward writes along is that of checkpoint8; the passes from it are those from the values it stands for."""
-    for i, act in enumerate(['relu', 'silu']):
+    """The checkpoint that the forward writes along is that of checkpoint8 with its codes on their elements' side of a ReLU's border; the passes from it are those
+    from the values it stands for, and take the forward's branch everywhere."""
+    for i, act in enumerate(['relu', 'silu', 'leaky', 'lin']):
         x, dy, w, b = make(size, dtype, seed=20 + i)
         y, mean, rstd, ck = ops.group_norm_act(x, size[5], w, b, activation=act, checkpoint=True)
         y2, mean2, rstd2 = ops.group_norm_act(x, size[5], w, b, activation=act)
         assert torch.equal(y, y2) and torch.equal(mean, mean2) and torch.equal(rstd, rstd2)
-        q, scale, val = ref_keep(x)
+        q, scale, _ = ref_keep(x)
+        q = ref_side(x, q, scale, mean, rstd, w, b, act)
+        val = (q.astype(np.float64) * np.repeat(scale.astype(np.float64), 64)[:q.size]).astype(np.float32)
         assert np.array_equal(ck.q.cpu().numpy(), q) and np.array_equal(ck.scale.cpu().numpy(), scale)
+        if act == 'relu' and scale.min() > 0:
+            ones = torch.ones_like(dy)
+            assert torch.equal(ops.group_norm_act_bwd(ck, mean, rstd, ones, w, b)[2], ops.group_norm_act_bwd(x, mean, rstd, ones, w, b)[2])
+        xin = x.clone()                                               # in place
+        y3, mean3, _, ck3 = ops.group_norm_act(xin, size[5], w, b, activation=act, checkpoint=True, out=xin)
+        assert y3 is xin and torch.equal(ck3.q, ck.q) and torch.equal(ck3.scale, ck.scale)
+        torch.testing.assert_close(mean3, mean, rtol=2 ** -22, atol=1e-7)
+        torch.testing.assert_close(y3, y, rtol=2 * HALF[dtype] + 1e-5, atol=1e-5)
         xt = torch.from_numpy(val).cuda().reshape(x.shape)            # fp32, whatever the type
         again = ops.group_norm_act_apply(ck, mean, rstd, w, b, activation=act)
         want, err = ref_fwd(xt, mean, rstd, w, b, act)
