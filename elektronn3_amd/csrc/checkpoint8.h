@@ -160,3 +160,8 @@ struct Border { int rule = 0; const float *mean = nullptr, *rstd = nullptr, *gam
 // launchers shared with the fused forms
 int launch_checkpoint8_pack(int dt, const void* x, int x_ldc, long long vox, int C, signed char* q, float* scale, const Border& border, hipStream_t s);
 int launch_checkpoint8_unpack(int dt, const signed char* q, const float* scale, long long vox, int C, void* y, int y_ldc, hipStream_t s);
+// the fp32 executor's: raw [N][D][H][W][C], a with rows of a_ldc, pooled (or nullptr) with windows of (kd, 2, 2)
+struct RestoreArgs {
+    const signed char* q; const float* qs; float* raw; const float *scale, *shift; float* a; int a_ldc; float* pooled; int kd; int N, D, H, W, C; ActArg act;
+};
+int launch_checkpoint8_act(const RestoreArgs& r, hipStream_t s);

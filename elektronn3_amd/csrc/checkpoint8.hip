@@ -22,15 +22,25 @@ template <int V, bool DENSE> __device__ __forceinline__ size_t piece_offset(size
     }
 }
 
-__device__ __forceinline__ bool positive(const Border& d, float x, size_t e, int C) {
-    const size_t v = e < 0xffffffffu ? (size_t)((unsigned)e / (unsigned)C) : e / (size_t)C;
-    const int c = (int)(e - v * (size_t)C);
-    if (d.rule == 2) return __builtin_fmaf(x, d.a[c], d.b[c]) > 0.f;
-    const size_t g = (v / (size_t)d.S) * d.G + c / (C / d.G);
-    return ((double)x - (double)d.mean[g]) * (double)d.rstd[g] * (d.gamma ? (double)d.gamma[c] : 1.0) + (d.beta ? (double)d.beta[c] : 0.0) > 0.0;
+// voxel v, channel c
+template <int RULE> __device__ __forceinline__ bool positive(const Border& d, float x, size_t g, int c) {
+    if constexpr (RULE == 2) return __builtin_fmaf(x, d.a[c], d.b[c]) > 0.f;
+    else return ((double)x - (double)d.mean[g]) * (double)d.rstd[g] * (d.gamma ? (double)d.gamma[c] : 1.0) + (d.beta ? (double)d.beta[c] : 0.0) > 0.0;
+}
+// codes of flat elements e0 ... moved to their side
+template <int RULE, int V> __device__ __forceinline__ void to_side(const Border& d, int C, size_t e0, const float (&f)[V], Codes<V>& q) {
+    size_t v = e0 < 0xffffffffu ? (size_t)((unsigned)e0 / (unsigned)C) : e0 / (size_t)C;
+    int c = (int)(e0 - v * (size_t)C);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        const size_t g = RULE == 1 ? (v / (size_t)d.S) * d.G + c / (C / d.G) : 0;
+        const float w = code_value<V>(q, e);
+        if (positive<RULE>(d, f[e], g, c) != positive<RULE>(d, w, g, c)) q.q[e] = other_neighbour(q.q[e], f[e], w);
+        if (++c == C) { c = 0; ++v; }
+    }
 }
 
-template <int DT, int V, bool DENSE, bool NT, bool SIDE>
+template <int DT, int V, bool DENSE, bool NT, int RULE>
 __global__ __launch_bounds__(BT) void checkpoint8_pack_kernel(const typename Elem<DT>::T* __restrict__ x, int ldc, int C, size_t n,
                                                               signed char* __restrict__ q, float* __restrict__ scale, const Border border) {
     constexpr int U = DT == DT_F32 ? 8 : 4;                  // pieces in flight per lane
@@ -51,14 +61,7 @@ __global__ __launch_bounds__(BT) void checkpoint8_pack_kernel(const typename Ele
             unpack_raw<DT, V>(raw[u], f);
             Codes<V> c = encode_block<V>(f);
             const size_t e0 = b0 + u * step + (size_t)threadIdx.x * V;
-            if constexpr (SIDE) {
-                if (ok[u] && c.scale > 0.f)
-#pragma unroll
-                    for (int e = 0; e < V; ++e) {
-                        const float v = code_value<V>(c, e);
-                        if (positive(border, f[e], e0 + e, C) != positive(border, v, e0 + e, C)) c.q[e] = other_neighbour(c.q[e], f[e], v);
-                    }
-            }
+            if constexpr (RULE != 0) if (ok[u] && c.scale > 0.f) to_side<RULE, V>(border, C, e0, f, c);
             if (ok[u]) store_codes<V>(c, q, scale, e0);
         }
     }
@@ -84,16 +87,63 @@ __global__ __launch_bounds__(BT) void checkpoint8_unpack_kernel(const signed cha
 
 constexpr size_t CACHE_BYTES = 256u << 20;
 
+// A unit's raw tensor out of its checkpoint together with what the executor forms from it: the activation a = act(fmaf(raw, scale, shift)) into a view and, POOL, its
+// ceil-mode max-pool -- the expressions and the order of elementwise.hip's passes, bit for bit.  One lane = one voxel (POOL: one window) x 4 channels.  (Restoring and
+// those passes one after the other read every raw tensor once more.)
+template <bool POOL>
+__global__ __launch_bounds__(BT) void checkpoint8_act_kernel(const RestoreArgs r) {
+    const float slope = r.act.get();
+    const int Q = r.C >> 2, kd = POOL ? r.kd : 1;
+    const int Dp = (r.D + kd - 1) / kd, Hp = POOL ? (r.H + 1) >> 1 : r.H, Wp = POOL ? (r.W + 1) >> 1 : r.W;
+    const size_t total = (size_t)r.N * Dp * Hp * Wp * Q;
+    auto one = [&](size_t v, int q, const RawQ<4>& raw) {
+        float f[4], o[4];
+        unpack_q<4>(raw, f);
+        const f32x4 sc = *reinterpret_cast<const f32x4*>(r.scale + 4 * q), sh = *reinterpret_cast<const f32x4*>(r.shift + 4 * q);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = act_fwd(__builtin_fmaf(f[e], sc[e], sh[e]), act_slope_at(r.act, slope, (unsigned)(v * r.C + 4 * q + e)));
+        *reinterpret_cast<f32x4*>(r.raw + v * r.C + 4 * q) = f32x4{f[0], f[1], f[2], f[3]};
+        const f32x4 y = {o[0], o[1], o[2], o[3]};
+        *reinterpret_cast<f32x4*>(r.a + v * r.a_ldc + 4 * q) = y;
+        return y;
+    };
+    for (size_t i = blockIdx.x * (size_t)BT + threadIdx.x; i < total; i += (size_t)gridDim.x * BT) {
+        const int q = i % Q; size_t t = i / Q;
+        if constexpr (!POOL) one(t, q, load_q<4>(r.q, r.qs, t * r.C + 4 * q));
+        else {
+            const int pw = t % Wp; t /= Wp; const int ph = t % Hp; t /= Hp; const int pd = t % Dp; const int n = t / Dp;
+            RawQ<4> raw[8]; size_t vox[8]; bool ok[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int dz = k >> 2, d = pd * kd + dz, h = ph * 2 + ((k >> 1) & 1), w = pw * 2 + (k & 1);
+                ok[k] = dz < kd && d < r.D && h < r.H && w < r.W;
+                vox[k] = (((size_t)n * r.D + d) * r.H + h) * r.W + w;
+                raw[k] = {};
+                if (ok[k]) raw[k] = load_q<4>(r.q, r.qs, vox[k] * r.C + 4 * q);
+            }
+            f32x4 best = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (ok[k]) {
+                    const f32x4 o = one(vox[k], q, raw[k]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) best[e] = (o[e] > best[e] || o[e] != o[e]) ? o[e] : best[e];
+                }
+            *reinterpret_cast<f32x4*>(r.pooled + ((((size_t)n * Dp + pd) * Hp + ph) * Wp + pw) * r.C + 4 * q) = best;
+        }
+    }
+}
+
 unsigned grid_for(size_t n, int V) {
     const size_t blocks = (n + (size_t)BT * V - 1) / ((size_t)BT * V);
     return (unsigned)(blocks < 2048 ? blocks : 2048);       // 8 workgroups of 4 waves per CU, grid-stride beyond
 }
 
-template <int DT, int V, bool NT, bool SIDE>
+template <int DT, int V, bool NT, int RULE>
 void pack_nt(const void* x, int ldc, size_t n, int C, signed char* q, float* scale, const Border& b, hipStream_t s) {
     typedef const typename Elem<DT>::T* P;
-    if (ldc == C) hipLaunchKernelGGL((checkpoint8_pack_kernel<DT, V, true, NT, SIDE>), dim3(grid_for(n, V)), dim3(BT), 0, s, (P)x, ldc, C, n, q, scale, b);
-    else hipLaunchKernelGGL((checkpoint8_pack_kernel<DT, V, false, NT, SIDE>), dim3(grid_for(n, V)), dim3(BT), 0, s, (P)x, ldc, C, n, q, scale, b);
+    if (ldc == C) hipLaunchKernelGGL((checkpoint8_pack_kernel<DT, V, true, NT, RULE>), dim3(grid_for(n, V)), dim3(BT), 0, s, (P)x, ldc, C, n, q, scale, b);
+    else hipLaunchKernelGGL((checkpoint8_pack_kernel<DT, V, false, NT, RULE>), dim3(grid_for(n, V)), dim3(BT), 0, s, (P)x, ldc, C, n, q, scale, b);
 }
 template <int DT, int V, bool NT>
 void unpack_nt(const signed char* q, const float* scale, size_t n, int C, void* y, int ldc, hipStream_t s) {
@@ -103,9 +153,10 @@ void unpack_nt(const signed char* q, const float* scale, size_t n, int C, void* 
 }
 template <int DT, int V>
 void pack_typed(const void* x, int ldc, size_t n, int C, signed char* q, float* scale, const Border& b, hipStream_t s) {
-    if (b.rule) pack_nt<DT, V, false, true>(x, ldc, n, C, q, scale, b, s);
-    else if (V > 1 && n * sizeof(typename Elem<DT>::T) >= CACHE_BYTES) pack_nt<DT, V, (V > 1), false>(x, ldc, n, C, q, scale, b, s);
-    else pack_nt<DT, V, false, false>(x, ldc, n, C, q, scale, b, s);
+    if (b.rule == 1) pack_nt<DT, V, false, 1>(x, ldc, n, C, q, scale, b, s);
+    else if (b.rule == 2 && DT == DT_F32) pack_nt<DT, V, false, DT == DT_F32 ? 2 : 0>(x, ldc, n, C, q, scale, b, s);      // (the fp32 executor's)
+    else if (V > 1 && n * sizeof(typename Elem<DT>::T) >= CACHE_BYTES) pack_nt<DT, V, (V > 1), 0>(x, ldc, n, C, q, scale, b, s);
+    else pack_nt<DT, V, false, 0>(x, ldc, n, C, q, scale, b, s);
 }
 template <int DT, int V>
 void unpack_typed(const signed char* q, const float* scale, size_t n, int C, void* y, int ldc, hipStream_t s) {
@@ -146,6 +197,18 @@ int launch_checkpoint8_unpack(int dt, const signed char* q, const float* scale, 
         case 4: unpack_typed<DT_F16, 1>(q, scale, n, C, y, y_ldc, s); break;
         default: unpack_typed<DT_F16, 8>(q, scale, n, C, y, y_ldc, s); break;
     }
+    E3_CHECK_HIP(hipGetLastError());
+    return E3_OK;
+}
+
+int launch_checkpoint8_act(const RestoreArgs& r, hipStream_t s) {
+    E3_REQUIRE(r.C % 4 == 0 && r.a_ldc % 4 == 0, E3_ERR_INVALID, "channel counts must be multiples of 4");
+    const int kd = r.pooled ? r.kd : 1;
+    const size_t items = (size_t)r.N * ((r.D + kd - 1) / kd) * (r.pooled ? (r.H + 1) / 2 : r.H) * (r.pooled ? (r.W + 1) / 2 : r.W) * (r.C / 4);
+    const size_t blocks = (items + BT - 1) / BT;
+    const dim3 grid((unsigned)(blocks < 4096 ? blocks : 4096));
+    if (r.pooled) hipLaunchKernelGGL(checkpoint8_act_kernel<true>, grid, dim3(BT), 0, s, r);
+    else hipLaunchKernelGGL(checkpoint8_act_kernel<false>, grid, dim3(BT), 0, s, r);
     E3_CHECK_HIP(hipGetLastError());
     return E3_OK;
 }

@@ -756,11 +756,13 @@ int e3_unet_checkpoint8_restore(const e3_unet_plan* plan, void* stream, int N, i
         const ConvUnit& u = plan->units[k];
         const UnitBufs& b = B.ub[k];
         const LevelDims& lo = ND.u[k].out;
-        RUN(launch_checkpoint8_unpack(E3_DT_F32, K.q[k], K.scale[k], (long long)lo.vox, u.cout, b.raw, u.cout, s));
-        if (k + 1 == plan->units.size()) break;        // (the head reads the raw tensor)
+        if (k + 1 == plan->units.size()) {             // (the head reads the raw tensor)
+            RUN(launch_checkpoint8_unpack(E3_DT_F32, K.q[k], K.scale[k], (long long)lo.vox, u.cout, b.raw, u.cout, s));
+            break;
+        }
         const ActArg act = plan->rrelu_of(u.p_a >= 0 ? ActArg(0.f, (const float*)params[u.p_a]) : ActArg(plan->cfg.act_slope), (int)k);
-        RUN(launch_bn_relu_apply(b.raw, u.cout, b.scale, b.shift, b.act, b.act_ldc, u.enc_last && u.level < nb - 1 ? B.pooled[u.level] : nullptr, u.planar ? 1 : 2,
-                                 N, lo.D, lo.H, lo.W, u.cout, s, act));
+        RUN(launch_checkpoint8_act({K.q[k], K.scale[k], b.raw, b.scale, b.shift, b.act, b.act_ldc, u.enc_last && u.level < nb - 1 ? B.pooled[u.level] : nullptr,
+                                    u.planar ? 1 : 2, N, lo.D, lo.H, lo.W, u.cout, act}, s));
         if (u.is_up && plan->cfg.merge_add)
             RUN(launch_add_views(B.cat[u.level], 2 * u.cout, B.cat[u.level] + u.cout, 2 * u.cout, B.sum[u.level], u.cout, lo.vox, u.cout, s));
     }
