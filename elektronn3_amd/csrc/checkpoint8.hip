@@ -22,21 +22,33 @@ template <int V, bool DENSE> __device__ __forceinline__ size_t piece_offset(size
     }
 }
 
-// voxel v, channel c
-template <int RULE> __device__ __forceinline__ bool positive(const Border& d, float x, size_t g, int c) {
-    if constexpr (RULE == 2) return __builtin_fmaf(x, d.a[c], d.b[c]) > 0.f;
-    else return ((double)x - (double)d.mean[g]) * (double)d.rstd[g] * (d.gamma ? (double)d.gamma[c] : 1.0) + (d.beta ? (double)d.beta[c] : 0.0) > 0.0;
-}
-// codes of flat elements e0 ... moved to their side
-template <int RULE, int V> __device__ __forceinline__ void to_side(const Border& d, int C, size_t e0, const float (&f)[V], Codes<V>& q) {
+// Codes of flat elements e0 ... moved to their side
+template <int V> __device__ __forceinline__ void to_side_exact(const Border& d, int C, size_t e0, const float (&f)[V], Codes<V>& q) {
     size_t v = e0 < 0xffffffffu ? (size_t)((unsigned)e0 / (unsigned)C) : e0 / (size_t)C;
     int c = (int)(e0 - v * (size_t)C);
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-        const size_t g = RULE == 1 ? (v / (size_t)d.S) * d.G + c / (C / d.G) : 0;
+        const size_t g = (v / (size_t)d.S) * d.G + c / (C / d.G);
+        const double mu = d.mean[g], rs = d.rstd[g], ga = d.gamma ? (double)d.gamma[c] : 1.0, be = d.beta ? (double)d.beta[c] : 0.0;
         const float w = code_value<V>(q, e);
-        if (positive<RULE>(d, f[e], g, c) != positive<RULE>(d, w, g, c)) q.q[e] = other_neighbour(q.q[e], f[e], w);
+        if ((((double)f[e] - mu) * rs * ga + be > 0.0) != (((double)w - mu) * rs * ga + be > 0.0)) q.q[e] = other_neighbour(q.q[e], f[e], w);
         if (++c == C) { c = 0; ++v; }
+    }
+}
+// ... with the constants a, b of a piece's channels (C % V == 0: a piece lies in one voxel)
+template <int V> struct Affine { float a[V], b[V]; };
+template <int V> __device__ __forceinline__ Affine<V> affine_at(const Border& d, int C, size_t e0) {
+    const int c = (int)(e0 < 0xffffffffu ? (unsigned)e0 % (unsigned)C : (unsigned)(e0 % (size_t)C));
+    Affine<V> k;
+#pragma unroll
+    for (int e = 0; e < V; ++e) { k.a[e] = d.a[c + e]; k.b[e] = d.b[c + e]; }
+    return k;
+}
+template <int V> __device__ __forceinline__ void to_side_affine(const Affine<V>& k, const float (&f)[V], Codes<V>& q) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        const float w = code_value<V>(q, e);
+        if ((__builtin_fmaf(f[e], k.a[e], k.b[e]) > 0.f) != (__builtin_fmaf(w, k.a[e], k.b[e]) > 0.f)) q.q[e] = other_neighbour(q.q[e], f[e], w);
     }
 }
 
@@ -45,6 +57,10 @@ __global__ __launch_bounds__(BT) void checkpoint8_pack_kernel(const typename Ele
                                                               signed char* __restrict__ q, float* __restrict__ scale, const Border border) {
     constexpr int U = DT == DT_F32 ? 8 : 4;                  // pieces in flight per lane
     const size_t step = (size_t)gridDim.x * BT * V;
+    // (where the grid's step is whole voxels a thread keeps its channels, and their constants)
+    const bool same = RULE == 2 && step % (size_t)C == 0;
+    Affine<V> k{};
+    if constexpr (RULE == 2) k = affine_at<V>(border, C, ((size_t)blockIdx.x * BT + threadIdx.x) * V);
     // (the loop's condition is the workgroup's: every lane of a wave reaches the reduction inside encode_block)
     for (size_t b0 = (size_t)blockIdx.x * BT * V; b0 < n; b0 += U * step) {
         Raw<DT, V> raw[U]; bool ok[U];
@@ -61,7 +77,11 @@ __global__ __launch_bounds__(BT) void checkpoint8_pack_kernel(const typename Ele
             unpack_raw<DT, V>(raw[u], f);
             Codes<V> c = encode_block<V>(f);
             const size_t e0 = b0 + u * step + (size_t)threadIdx.x * V;
-            if constexpr (RULE != 0) if (ok[u] && c.scale > 0.f) to_side<RULE, V>(border, C, e0, f, c);
+            if constexpr (RULE == 1) if (ok[u] && c.scale > 0.f) to_side_exact<V>(border, C, e0, f, c);
+            if constexpr (RULE == 2) if (ok[u] && c.scale > 0.f) {
+                if (!same) k = affine_at<V>(border, C, e0);
+                to_side_affine<V>(k, f, c);
+            }
             if (ok[u]) store_codes<V>(c, q, scale, e0);
         }
     }
@@ -154,7 +174,7 @@ void unpack_nt(const signed char* q, const float* scale, size_t n, int C, void* 
 template <int DT, int V>
 void pack_typed(const void* x, int ldc, size_t n, int C, signed char* q, float* scale, const Border& b, hipStream_t s) {
     if (b.rule == 1) pack_nt<DT, V, false, 1>(x, ldc, n, C, q, scale, b, s);
-    else if (b.rule == 2 && DT == DT_F32) pack_nt<DT, V, false, DT == DT_F32 ? 2 : 0>(x, ldc, n, C, q, scale, b, s);      // (the fp32 executor's)
+    else if (b.rule == 2) pack_nt<DT, V, false, V == 4 ? 2 : 0>(x, ldc, n, C, q, scale, b, s);        // (the fp32 executor's)
     else if (V > 1 && n * sizeof(typename Elem<DT>::T) >= CACHE_BYTES) pack_nt<DT, V, (V > 1), 0>(x, ldc, n, C, q, scale, b, s);
     else pack_nt<DT, V, false, 0>(x, ldc, n, C, q, scale, b, s);
 }
@@ -174,6 +194,8 @@ bool wide(int dt, const void* p, int ldc, int C, size_t n, const void* q) {
 int launch_checkpoint8_pack(int dt, const void* x, int x_ldc, long long vox, int C, signed char* q, float* scale, const Border& border, hipStream_t s) {
     const size_t n = (size_t)vox * C;
     if (n == 0) return E3_OK;
+    E3_REQUIRE(border.rule != 2 || (dt == DT_F32 && C % 4 == 0 && x_ldc == C && wide(dt, x, x_ldc, C, n, q) && aligned16(border.a) && aligned16(border.b)), E3_ERR_INVALID,
+               "a checkpoint with channel constants: packed fp32 tensor with 16-byte rows expected");
     switch (dt * 2 + wide(dt, x, x_ldc, C, n, q)) {
         case 0: pack_typed<DT_F32, 1>(x, x_ldc, n, C, q, scale, border, s); break;
         case 1: pack_typed<DT_F32, 4>(x, x_ldc, n, C, q, scale, border, s); break;
