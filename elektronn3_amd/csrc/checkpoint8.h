@@ -165,3 +165,4 @@ struct RestoreArgs {
     const signed char* q; const float* qs; float* raw; const float *scale, *shift; float* a; int a_ldc; float* pooled; int kd; int N, D, H, W, C; ActArg act;
 };
 int launch_checkpoint8_act(const RestoreArgs& r, hipStream_t s);
+int launch_checkpoint8_windows(const RestoreArgs& r, signed char* codes, bool side, hipStream_t s);      // (reads r.raw; r.q, r.a, r.pooled are not used)

@@ -701,6 +701,10 @@ void kept8_layout(const e3_unet_plan* p, const NetDims& ND, void* base, Kept8& K
     }
     K.bytes = A.off;
 }
+ActArg activation_of(const e3_unet_plan* p, void* const* params, size_t k) {
+    const ConvUnit& u = p->units[k];
+    return p->rrelu_of(u.p_a >= 0 ? ActArg(0.f, (const float*)params[u.p_a]) : ActArg(p->cfg.act_slope), (int)k);
+}
 // what both directions check and lay out
 int kept8_open(const e3_unet_plan* plan, int N, int D, int H, int W, void* saved, size_t saved_bytes, void* kept, size_t kept_bytes, NetDims& ND, Buffers& B, Kept8& K) {
     E3_REQUIRE(plan && N > 0 && D > 0 && H > 0 && W > 0 && saved && kept, E3_ERR_INVALID, "bad argument");
@@ -725,7 +729,9 @@ int e3_unet_checkpoint8_bytes(const e3_unet_plan* plan, int N, int D, int H, int
     return E3_OK;
 }
 
-int e3_unet_checkpoint8_keep(const e3_unet_plan* plan, void* stream, int N, int D, int H, int W, const void* saved, size_t saved_bytes, void* kept, size_t kept_bytes) {
+int e3_unet_checkpoint8_keep(const e3_unet_plan* plan, void* stream, int N, int D, int H, int W, void* const* params, const void* saved, size_t saved_bytes,
+                             void* kept, size_t kept_bytes) {
+    E3_REQUIRE(params, E3_ERR_INVALID, "null argument");
     NetDims ND; Buffers B; Kept8 K;
     RUN(kept8_open(plan, N, D, H, W, const_cast<void*>(saved), saved_bytes, kept, kept_bytes, ND, B, K));
     hipStream_t s = (hipStream_t)stream;
@@ -735,6 +741,11 @@ int e3_unet_checkpoint8_keep(const e3_unet_plan* plan, void* stream, int N, int 
         Border side;          // (the rounded tensors take the forward's branch of every ReLU)
         if (plan->cfg.act_slope != 1.f && plan->cfg.act_slope != ACT_SILU) { side.rule = 2; side.a = B.ub[k].scale; side.b = B.ub[k].shift; }
         RUN(launch_checkpoint8_pack(E3_DT_F32, B.ub[k].raw, C, (long long)ND.u[k].out.vox, C, K.q[k], K.scale[k], side, s));
+        if (plan->units[k].enc_last && plan->units[k].level < plan->cfg.n_blocks - 1) {       // (... and hand every pooled gradient to the forward's voxel)
+            const LevelDims& lo = ND.u[k].out;
+            RUN(launch_checkpoint8_windows({nullptr, K.scale[k], B.ub[k].raw, B.ub[k].scale, B.ub[k].shift, nullptr, 0, nullptr, plan->units[k].planar ? 1 : 2, N, lo.D, lo.H, lo.W, C,
+                                            activation_of(plan, params, k)}, K.q[k], side.rule != 0, s));
+        }
         copies.push_back({B.ub[k].mean, K.vec[k], vec_floats(C)});
     }
     if (K.xin_floats) copies.push_back({B.xin, K.xin, K.xin_floats});
@@ -760,7 +771,7 @@ int e3_unet_checkpoint8_restore(const e3_unet_plan* plan, void* stream, int N, i
             RUN(launch_checkpoint8_unpack(E3_DT_F32, K.q[k], K.scale[k], (long long)lo.vox, u.cout, b.raw, u.cout, s));
             break;
         }
-        const ActArg act = plan->rrelu_of(u.p_a >= 0 ? ActArg(0.f, (const float*)params[u.p_a]) : ActArg(plan->cfg.act_slope), (int)k);
+        const ActArg act = activation_of(plan, params, k);
         RUN(launch_checkpoint8_act({K.q[k], K.scale[k], b.raw, b.scale, b.shift, b.act, b.act_ldc, u.enc_last && u.level < nb - 1 ? B.pooled[u.level] : nullptr,
                                     u.planar ? 1 : 2, N, lo.D, lo.H, lo.W, u.cout, act}, s));
         if (u.is_up && plan->cfg.merge_add)

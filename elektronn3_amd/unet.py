@@ -137,14 +137,15 @@ class _Kept8:
     """The `saved` arena of a training forward in 8 bits (e3_unet_checkpoint8_keep / _restore): what the autograd node holds with ``UNet.checkpoint8()``."""
     __slots__ = ('plan', 'dims', 'buf', 'nbytes')
 
-    def __init__(self, plan, dims, saved):
+    def __init__(self, plan, dims, saved, tens):
         lib = _lib.load()
         n = c_size_t()
         check(lib.e3_unet_checkpoint8_bytes(plan.handle, *dims, ctypes.byref(n)))
         self.plan, self.dims, self.nbytes = plan, dims, saved.numel()
         self.buf = torch.empty(n.value, dtype=torch.uint8, device=saved.device)
+        ptrs = (c_void_p * len(tens))(*[t.data_ptr() for t in tens])
         with torch.cuda.device(saved.device):
-            check(lib.e3_unet_checkpoint8_keep(plan.handle, _lib.stream_ptr(saved.device), *dims, c_void_p(saved.data_ptr()), c_size_t(saved.numel()),
+            check(lib.e3_unet_checkpoint8_keep(plan.handle, _lib.stream_ptr(saved.device), *dims, ptrs, c_void_p(saved.data_ptr()), c_size_t(saved.numel()),
                                                c_void_p(self.buf.data_ptr()), c_size_t(self.buf.numel())))
 
     def restore(self, tens):
@@ -451,7 +452,7 @@ class _UNetFunction(torch.autograd.Function):
         # (a low-precision module's fp32 table is a cache that the next forward refreshes with the same parameter values:
         # the backward only reads weights and affine parameters from it, never the running statistics)
         if need_grad and module.__dict__.get('_checkpoint8'):
-            saved = _Kept8(plan, (xin.shape[0], *xin.shape[2:]), saved)
+            saved = _Kept8(plan, (xin.shape[0], *xin.shape[2:]), saved, tens)
         ctx.x32, ctx.saved_buf, ctx.tens = (xin, saved, _TableRef(tens, False)) if need_grad else (None, None, None)
         if need_grad and lowp is not None:
             # the fp32 table of a low-precision module is ONE persistent cache that the next forward overwrites in place: this forward registers its
@@ -1270,7 +1271,7 @@ class UNet(nn.Module):
         ``normalization='group'`` / ``'instance'``, whose batch is one graph per sample.  The outputs are unchanged; the gradients are those of the rounded
         tensors: of every norm's input, an element is off by at most 1/254 of the largest of its block of 64 (:class:`elektronn3_amd.ops.Checkpoint8`),
         and the activations are recomputed from them.  What the reference's ``forward_gradcp`` (unet.py:918-935) trades recomputation for, this trades
-        precision for.  fp32 compute; transposed up-convolutions, 'same' convolutions and a norm behind every convolution, no attention
+        precision for.  The rounding keeps every element on its side of a ReLU's border and every pooling window's maximum in place.  fp32 compute; transposed up-convolutions, 'same' convolutions and a norm behind every convolution, no attention
         (NotImplementedError otherwise).  Scripted modules keep their activations as they are.  Returns the module."""
         if enabled:
             n = c_size_t()

@@ -14,8 +14,9 @@ pytestmark = pytest.mark.gpu
 TOL = 2e-3
 
 
-def kept(x, z, border):
-    """What the 8-bit checkpoint of an NCDHW tensor stands for (blocks of 64 of the NDHWC order); border: rounded to the side of z = 0 that an element is on."""
+def kept(x, z, border, pool=None, fn=None):
+    """What the 8-bit checkpoint of an NCDHW tensor stands for (blocks of 64 of the NDHWC order); border: rounded to the side of z = 0 that an element is on;
+    pool: window of the max-pool behind fn(z), whose first maximum stays where it is."""
     v = x.detach().float().movedim(1, -1).contiguous()
     flat = v.reshape(-1).numpy()
     p = np.zeros(-(-flat.size // 64) * 64, np.float32); p[:flat.size] = flat
@@ -28,8 +29,39 @@ def kept(x, z, border):
         move = torch.where((z(x) > 0) != (z(val) > 0), torch.where(x > val, 1.0, -1.0), 0.0).movedim(1, -1).reshape(-1).numpy()
         p[:] = 0
         p.reshape(-1)[:flat.size] = move
-        val = back(np.clip(q + p, -127, 127))
+        q = np.clip(q + p, -127, 127)
+        val = back(q)
+    if pool:
+        step = torch.where(x > val, 1.0, -1.0).movedim(1, -1).reshape(-1).numpy()
+        p[:] = 0
+        p.reshape(-1)[:flat.size] = step
+        val = windows(x, val, back(np.clip(q + p, -127, 127)), z, fn, border, pool)
     return val
+
+
+def windows(x, v0, v1, z, fn, border, pool):
+    """v0, v1: the two neighbours of x on the grid of its block, v0 the one in use.  Per window: the maximum of fn(z(x)) takes the larger of its two where the rounded
+    values have another maximum, then what still reaches it the smaller of its two."""
+    def cut(t, fill):
+        t = torch.nn.functional.pad(t, [n for s, k in zip(t.shape[:1:-1], pool[::-1]) for n in (0, -s % k)], value=fill)
+        return torch.stack([t[:, :, d::pool[0], h::2, w::2] for d in range(pool[0]) for h in range(2) for w in range(2)])
+    ok = cut(torch.ones_like(x), 0) > 0
+    inf = torch.tensor(float('-inf'), dtype=torch.float64)
+    o, o0, o1 = (torch.where(ok, cut(fn(z(t)), 0), inf) for t in (x, v0, v1))
+    allowed = ok & (cut(((z(v0) > 0) == (z(v1) > 0)).double(), 0) > 0) if border else ok
+    first = lambda t: (t == t.max(0, keepdim=True).values).double().argmax(0, keepdim=True)      # noqa: E731
+    m, wrong = first(o), first(o) != first(o0)
+    k = torch.arange(o.shape[0]).view(-1, 1, 1, 1, 1, 1)
+    take = wrong & (k == m) & allowed & (o1 > o0)
+    now = torch.where(take, o1, o0)
+    top = now.gather(0, m)
+    reach = torch.where(k < m, now >= top, now > top) & (k != m)
+    take = take | (wrong & reach & allowed & (o1 < o0))
+    out = torch.where(take, cut(v1, 0), cut(v0, 0))
+    full = torch.zeros(*x.shape[:2], *(n * s for n, s in zip(out.shape[3:], pool)), dtype=torch.float64)
+    for i, t in enumerate(out):
+        full[:, :, i // 4::pool[0], i // 2 % 2::2, i % 2::2] = t
+    return full[:, :, :x.shape[2], :x.shape[3], :x.shape[4]]
 
 
 class Norm(torch.autograd.Function):
@@ -61,7 +93,7 @@ def emulate(m, x, dy, act, groups=None, add=False, replace=True, frozen=False):
     if flat:
         x, dy = x.unsqueeze(2), dy.unsqueeze(2)
 
-    def unit(conv, a, a_exact, prefix, norm, up=False, slope=None):
+    def unit(conv, a, a_exact, prefix, norm, up=False, slope=None, pool=None):
         w, b = sd[f'{prefix}.weight'], sd[f'{prefix}.bias']
         w = w.unsqueeze(2) if flat else w
         k = tuple(w.shape[2:])
@@ -79,13 +111,13 @@ def emulate(m, x, dy, act, groups=None, add=False, replace=True, frozen=False):
         inv = 1 / (var + 1e-5).sqrt()
         ga, be = (sd[f'{norm}.weight'], sd[f'{norm}.bias']) if groups != 0 else (torch.ones(raw.shape[1], dtype=torch.float64), torch.zeros(raw.shape[1], dtype=torch.float64))
         aff = lambda t: ((t - mean) * inv * ga.view(1, -1, 1, 1, 1) + be.view(1, -1, 1, 1, 1)).detach()    # noqa: E731
-        y = y + ((kept(raw, aff, act not in ('silu', 'lin')) if replace else raw) - y).detach()
+        fn = {'relu': F.relu, 'leaky': lambda t: F.leaky_relu(t, 0.1), 'leaky2': lambda t: F.leaky_relu(t, 0.2), 'silu': F.silu, 'prelu': lambda t: F.prelu(t, sd[slope])}[act]
+        y = y + ((kept(raw, aff, act not in ('silu', 'lin'), pool, lambda t: fn(t).detach()) if replace else raw) - y).detach()
         if frozen:
             z = (y - mean) * inv * ga.view(1, -1, 1, 1, 1) + be.view(1, -1, 1, 1, 1)
         else:
             z = Norm.apply(y, ga, be, mean, inv, G)
         ze = aff(raw)
-        fn = {'relu': F.relu, 'leaky': lambda t: F.leaky_relu(t, 0.1), 'leaky2': lambda t: F.leaky_relu(t, 0.2), 'silu': F.silu, 'prelu': lambda t: F.prelu(t, sd[slope])}[act]
         return fn(z), fn(ze).detach()
 
     a = ae = x.cpu().double()
@@ -93,7 +125,8 @@ def emulate(m, x, dy, act, groups=None, add=False, replace=True, frozen=False):
     nb = len(m.down_convs)
     for i in range(nb):
         for c in (1, 2):
-            a, ae = unit(None, a, ae, f'down_convs.{i}.conv{c}', f'down_convs.{i}.norm{c - 1}', slope=f'down_convs.{i}.act{c}.weight')
+            a, ae = unit(None, a, ae, f'down_convs.{i}.conv{c}', f'down_convs.{i}.norm{c - 1}', slope=f'down_convs.{i}.act{c}.weight',
+                         pool=(1 if flat or i in m.planar_blocks else 2, 2, 2) if c == 2 and i < nb - 1 else None)
         if i < nb - 1:
             skips.append((a, ae))
             a, ae = (F.max_pool3d(t, (1, 2, 2) if flat or i in m.planar_blocks else 2, ceil_mode=True) for t in (a, ae))
@@ -143,8 +176,9 @@ def test_gradients_are_those_of_the_rounded_tensors(kw, shape, act):
     m.checkpoint8()
     out8 = check(m, x, dy, emulate(m, x, dy, act, groups, add))
     want, plain = emulate(m, x, dy, act, groups, add), emulate(m, x, dy, act, groups, add, replace=False)
-    moved = [float((plain[k] - w).norm()) > 2 * TOL * float(w.norm()) for k, w in want.items() if counts(k)]
-    assert sum(moved) > len(moved) // 3, 'the checkpoints make no difference: nothing is tested'
+    change = [float((plain[k] - w).norm()) / float(w.norm()) for k, w in want.items() if counts(k)]
+    print('change of the gradients: median %.2g, largest %.2g' % (sorted(change)[len(change) // 2], max(change)))
+    assert sum(c > TOL for c in change) > len(change) // 3, 'the checkpoints make no difference: nothing is tested'
     # the outputs do not change, and switched off the gradients are the full ones again
     m.checkpoint8(False)
     assert torch.equal(check(m, x, dy, plain), out8)
