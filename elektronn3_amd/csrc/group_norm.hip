@@ -218,7 +218,7 @@ __device__ __forceinline__ void keep_side(const GnArgs& a, int c, const float (&
 }
 
 // ------------------------------------------------------------------------------------------------ forward
-// Sums and sums of squares in fp64: the variance is then a difference that loses nothing an fp32 input holds, whatever its mean.
+// Sums and sums of squares in fp64: the variance is then a difference that is off by 1e-16 (mean / std)^2 -- less than the inputs' own rounding up to mean / std = 1e5.
 template <int V, int UN> struct Moments {
     double s[V / UN], t[V / UN];
     __device__ __forceinline__ Moments() {
@@ -411,7 +411,7 @@ __device__ __forceinline__ void grad_piece(const GnArgs& a, int n, int c, const 
         }
     }
 }
-// Per-thread sums of dz and dz t (h = t rstd: the factor comes last) in fp32 over at most a chunk's voxels / R, everything behind them in fp64.
+// Per-thread sums of dz and dz t (h = t rstd: the factor comes last) in fp32 over at most SUM_TERMS elements, everything behind them in fp64.
 template <int DT, int V, int UN, bool CK, bool SILU>
 __global__ __launch_bounds__(MAX_T) void gn_bwd_reduce_kernel(const GnArgs a) {
     extern __shared__ float shf[];
@@ -562,11 +562,12 @@ struct Shape { int N; long long S; int C, G; };
 
 constexpr int PASS_WGS = 512;                // workgroups of a pass: two per CU (256 threads each); 1024 cost the merges of mid-sized tensors 2 - 8 us and gain nothing
 constexpr int PASS_T = 256;
+constexpr int SUM_TERMS = 512;               // fp32 terms of a sum: their rounding stays below 512 2^-24 of the sum of magnitudes, with more chunks for samples of more voxels
 
 void set_shape(GnArgs& a, const Shape& sh) { a.N = sh.N; a.S = sh.S; a.C = sh.C; a.G = sh.G; a.cg = sh.C / sh.G; a.inv_m = 1.0 / ((double)sh.S * a.cg); }
 
-// mapping of a pass; `target`: workgroups that it asks for (at least one per sample and tile)
-template <int V> void map_pass(GnArgs& a, const Shape& sh, int target, int U, bool keep) {
+// mapping of a pass; `target`: workgroups that it asks for (at least one per sample and tile); `terms`: voxels of a thread at most, or 0
+template <int V> void map_pass(GnArgs& a, const Shape& sh, int target, int U, bool keep, int terms = 0) {
     set_shape(a, sh);
     a.P = sh.C / V;
     a.tiles = (a.P + MAX_T - 1) / MAX_T;
@@ -579,6 +580,7 @@ template <int V> void map_pass(GnArgs& a, const Shape& sh, int target, int U, bo
     }
     long long most = target / ((long long)sh.N * a.tiles);
     if (most < 1) most = 1;
+    if (terms && most < (sh.S + (long long)terms * a.R - 1) / ((long long)terms * a.R)) most = (sh.S + (long long)terms * a.R - 1) / ((long long)terms * a.R);
     const long long step = (long long)a.R * U;
     long long chunks = (sh.S + step - 1) / step;
     if (chunks > most) chunks = most;
@@ -622,7 +624,7 @@ template <int V> size_t space_of(const Shape& sh, bool backward) {
     if (sh.C % V != 0) return 0;
     GnArgs a{};
     if (!backward) return map_group<V>(a, sh) ? 0 : fwd_part_doubles<V>(sh) * sizeof(double);
-    map_pass<V>(a, sh, PASS_WGS, U2<V>, false);
+    map_pass<V>(a, sh, PASS_WGS, U2<V>, false, SUM_TERMS);
     const BwdSpace b = bwd_space(a, sh);
     return b.channels + b.behind;
 }
@@ -705,7 +707,7 @@ template <int DT, int V, int UN> int forward(GnArgs a, const Shape& sh, void* ws
 
 template <int DT, int V, int UN, bool CK> int backward(GnArgs a, const Shape& sh, void* ws, hipStream_t s) {
     GnArgs st = a;
-    map_pass<V>(st, sh, PASS_WGS, U2<V>, false);
+    map_pass<V>(st, sh, PASS_WGS, U2<V>, false, SUM_TERMS);
     st.part = (double*)ws;
     const BwdSpace space = bwd_space(st, sh);
     void* behind = (char*)ws + space.channels;
@@ -753,7 +755,8 @@ int check_shape(int dtype, int N, int D, int H, int W, int C, int G, float slope
     E3_REQUIRE(G >= 1 && C % G == 0, E3_ERR_INVALID, "num_groups must divide the channel count");
     E3_REQUIRE(act_ok(slope), E3_ERR_UNSUPPORTED, "activation slope must be in [0, 1], or 2 for SiLU");
     sh.N = N; sh.S = (long long)D * H * W; sh.C = C; sh.G = G;
-    E3_REQUIRE((long long)N * ((C + MAX_T - 1) / MAX_T) <= (1ll << 30) && (long long)N * G + C < (1ll << 31), E3_ERR_UNSUPPORTED, "too many samples");
+    // (a launch has fewer than 2^32 threads: 512 per group or tile, 256 per 16 channels)
+    E3_REQUIRE((long long)N * G < (1ll << 23) && (long long)N * ((C + MAX_T - 1ll) / MAX_T) < (1ll << 23) && C <= (1 << 26), E3_ERR_UNSUPPORTED, "more than 2^23 groups or 2^26 channels");
     return E3_OK;
 }
 

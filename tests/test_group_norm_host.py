@@ -110,3 +110,10 @@ def test_workspace_sizes(dims):
     assert call('e3_group_norm_workspace_bytes', *dims[:5], dims[5] + dims[4] + 1, 1) == 0
     # the forward of small groups needs none
     assert call('e3_group_norm_workspace_bytes', 1, 4, 8, 8, 128, 8, 0) == 0 < call('e3_group_norm_workspace_bytes', 1, 64, 64, 64, 128, 8, 0)
+
+
+def test_sums_of_long_samples_are_cut():
+    """A thread's fp32 sums of the backward have at most 512 terms: 256 threads to a workgroup, one (sum, sum) record of doubles per workgroup and channel."""
+    voxels = 16384 * 16384
+    assert call('e3_group_norm_workspace_bytes', 1, 1, 16384, 16384, 1, 1, 1) >= voxels // (512 * 256) * 16
+    assert call('e3_group_norm_workspace_bytes', 1, 1, 16384, 16384, 32, 8, 1) >= voxels // (512 * 64) * 32 * 16
