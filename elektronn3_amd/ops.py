@@ -30,6 +30,8 @@ def _ldc(t):
         and (N == 1 or sN == D * H * W * ldc or (D == 1 and H == 1 and W == 1))
     if not ok:
         raise ValueError(f'not an NDHWC view: shape {tuple(t.shape)} strides {t.stride()}')
+    if ldc >= 1 << 31:
+        raise ValueError(f'rows of {ldc} elements: longer than the kernels address')
     return ldc
 
 

@@ -117,3 +117,12 @@ def test_sums_of_long_samples_are_cut():
     voxels = 16384 * 16384
     assert call('e3_group_norm_workspace_bytes', 1, 1, 16384, 16384, 1, 1, 1) >= voxels // (512 * 256) * 16
     assert call('e3_group_norm_workspace_bytes', 1, 1, 16384, 16384, 32, 8, 1) >= voxels // (512 * 64) * 32 * 16
+
+
+def test_rows_and_groups_beyond_the_kernels():
+    t = torch.empty(8, device='meta').as_strided((2, 1, 1, 1, 8), (1 << 31, 8, 8, 8, 1))
+    with pytest.raises(ValueError, match='rows of'):
+        ops._ldc(t)
+    lib = _lib.load()
+    rc = lib.e3_group_norm_act_fwd(None, 0, FAKE, 32, None, None, 1e-5, 0.0, FAKE, 32, FAKE, FAKE, None, None, 1 << 20, 1, 1, 1, 32, 8, None, 0)
+    assert rc == 3 and b'groups' in lib.e3_last_error()
