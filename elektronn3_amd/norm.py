@@ -73,7 +73,7 @@ class GroupNormAct(nn.GroupNorm):
             raise ValueError(f'expected {self.num_channels} channels, got {x.shape[1]}')
         if not x.is_cuda:
             raise RuntimeError('elektronn3_amd.GroupNormAct runs only on a ROCm GPU (hand-written HIP kernels); there is no CPU fallback')
-        return _GroupNormActFunction.apply(x, self.weight, self.bias, self.num_groups, self.eps, self.activation, self.checkpoint)
+        return _GroupNormActFunction.apply(x, self.weight, self.bias, self.num_groups, self.eps, self.activation, self.checkpoint and torch.is_grad_enabled())
 
     def extra_repr(self):
         return super().extra_repr() + f', activation={self.activation!r}, checkpoint={self.checkpoint}'

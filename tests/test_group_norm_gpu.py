@@ -428,6 +428,74 @@ def test_other_stream_and_two_graphs_replayed(ops):
             assert all(torch.equal(p, q) for p, q in zip(outs, step())), rep
 
 
+def test_two_calls_at_once(ops):
+    """Two threads, each on a stream of its own, each with its own workspaces: the results of one after the other."""
+    import threading
+    data = [make((2, 6, 16, 17, 64, 8), torch.float16, seed=70 + k) for k in range(2)]
+
+    def step(d):
+        x, dy, w, b = d
+        y, mean, rstd, ck = ops.group_norm_act(x, 8, w, b, checkpoint=True)
+        return (y, *ops.group_norm_act_bwd(ck, mean, rstd, dy, w, b), ops.checkpoint8_restore(ck))
+    want = [step(d) for d in data]
+    torch.cuda.synchronize()
+    got = [None, None]
+
+    def work(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got[k] = step(data[k])
+            torch.cuda.current_stream().synchronize()
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for g, r in zip(got, want):
+        assert all(torch.equal(p, q) for p, q in zip(g, r))
+
+
+def test_offsets_past_32_bits(ops):
+    """A batch of 4.3e9 elements: its last sample, whose offsets do not fit 32 bits, gives what it gives alone."""
+    if torch.cuda.get_device_properties(0).total_memory < 100 << 30:
+        pytest.skip('needs 100 GB')
+    shape = (2, 1, 8200, 8200, 32)
+    x = torch.empty(shape, dtype=torch.bfloat16, device='cuda')
+    g = torch.Generator(device='cuda').manual_seed(1)
+    tile = torch.randn(8200, 32, device='cuda', generator=g) + 0.5
+    for n in range(2):                       # rows of one tile, scaled: every row of every sample is different
+        x[n, 0] = (tile[None] * torch.linspace(0.5 + n, 1.5 + n, 8200, device='cuda')[:, None, None]).to(torch.bfloat16)
+    w, b = torch.ones(32, device='cuda'), torch.full((32,), 0.1, device='cuda')
+    y, mean, rstd, ck = ops.group_norm_act(x, 8, w, b, checkpoint=True)
+    y1, mean1, rstd1, ck1 = ops.group_norm_act(x[1:], 8, w, b, checkpoint=True)
+    torch.testing.assert_close(mean[1:], mean1, rtol=2 ** -22, atol=0)
+    torch.testing.assert_close(y[1:, :, -3:], y1[:, :, -3:], rtol=2 ** -7, atol=1e-5)
+    n = x[0].numel()
+    assert torch.equal(ck.scale[n // 64:], ck1.scale) and float((ck.q[n:] != ck1.q).float().mean()) < 1e-6      # (codes at the border go by the statistics' last bit)
+    back = ops.checkpoint8_restore(ck)
+    assert torch.equal(back[1:, :, -3:], ops.checkpoint8_restore(ops.Checkpoint8(ck.q[n:], ck.scale[n // 64:], x[1:].shape, x.dtype))[:, :, -3:])
+    del back, y, y1
+    dx, _, _ = ops.group_norm_act_bwd(ck, mean, rstd, x, w, b)
+    dx1, _, _ = ops.group_norm_act_bwd(ops.Checkpoint8(ck.q[n:], ck.scale[n // 64:], x[1:].shape, x.dtype), mean[1:], rstd[1:], x[1:], w, b)
+    torch.testing.assert_close(dx[1:, :, -3:], dx1[:, :, -3:], rtol=2 ** -6, atol=1e-3)
+
+
+def test_gradient_written_over_its_source(ops):
+    """The C entry's dx may be dy, and a NULL dgamma or dbeta is left out."""
+    from elektronn3_amd import _lib
+    for shape, dt in (((2, 5, 9, 16, 32, 8), torch.bfloat16), ((1, 3, 7, 5, 24, 3), torch.float32), ((2, 3, 7, 5, 7, 7), torch.float16), ((1, 2, 3, 4, 2048, 256), torch.float32)):
+        x, dy, w, b = make(shape, dt, seed=3)
+        y, mean, rstd = ops.group_norm_act(x, shape[5], w, b)
+        dx, dw, db = ops.group_norm_act_bwd(x, mean, rstd, dy, w, b)
+        g, dw2 = dy.clone(), torch.empty_like(dw)
+        L = _lib.load()
+        ws = torch.empty(L.e3_group_norm_workspace_bytes(*shape, 1), dtype=torch.uint8, device='cuda')
+        C = shape[4]
+        _lib.check(L.e3_group_norm_act_bwd(_lib.stream_ptr(x.device), ops._DT[dt], x.data_ptr(), C, None, None, mean.data_ptr(), rstd.data_ptr(), w.data_ptr(), b.data_ptr(), 0.0,
+                                           g.data_ptr(), C, g.data_ptr(), C, dw2.data_ptr(), None, *shape, ws.data_ptr(), ws.numel()))
+        assert torch.equal(g, dx) and torch.equal(dw2, dw)
+
+
 # ------------------------------------------------------------------------------------------------ module
 @pytest.mark.parametrize('checkpoint', [False, True])
 @pytest.mark.parametrize('dtype', DTYPES)
@@ -463,6 +531,43 @@ def test_module(dims, dtype, checkpoint):
         lim = tol if not checkpoint else 0.05
         for a, r in ((x.grad, xr.grad), (m.weight.grad, ref.weight.grad), (m.bias.grad, ref.bias.grad)):
             assert float((a.cpu().double() - r).norm()) <= lim * float(r.norm()) + 1e-6
+
+
+def test_module_captured_with_its_backward():
+    """Forward and backward of a small network captured into a graph; replays, with eager work in between, give the eager gradients."""
+    from elektronn3_amd.norm import GroupNormAct
+    torch.manual_seed(1)
+    m = torch.nn.Sequential(GroupNormAct(2, 16, checkpoint=True), GroupNormAct(4, 16, activation='silu')).cuda()
+    x = torch.randn(2, 16, 5, 8, 9, device='cuda').contiguous(memory_format=torch.channels_last_3d)
+    dy = torch.randn_like(x)
+    params = list(m.parameters())
+
+    def step():
+        return torch.autograd.grad(m(x), params, dy)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        outs = step()
+    for rep in range(4):
+        x.copy_(torch.randn_like(x)); dy.copy_(torch.randn_like(dy))
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, step())), rep
+
+
+def test_module_keeps_nothing_without_gradients(monkeypatch):
+    from elektronn3_amd import ops as o
+    from elektronn3_amd.norm import GroupNormAct
+    m, x = GroupNormAct(2, 16, checkpoint=True).cuda(), torch.randn(1, 16, 3, 4, 5, device='cuda')
+    y = m(x)
+    monkeypatch.setattr(o, '_new_checkpoint', lambda x: pytest.fail('a checkpoint without a backward'))
+    with torch.no_grad():
+        assert torch.equal(m(x), y)
 
 
 def test_module_inside_a_network_and_its_state_dict():
