@@ -335,12 +335,13 @@ def convT_wgrad_bf16(x, dy):
 # (small calls are bound by this file: a forward is two launches of 4 us, so the checks below look at every property once and tensors are allocated once)
 _DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}       # E3_DT_*
 _SLOPES = {'relu': 0.0, 'leaky': 0.1, 'lin': 1.0, 'silu': 2.0}
+_current_device = getattr(torch._C, '_cuda_getDevice', None) or torch.cuda.current_device
 _raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _call(device, fn, *args):
     """One native call on the tensors' device and its current stream."""
-    if torch.cuda.current_device() == device.index:
+    if _current_device() == device.index:
         rc = fn(_raw_stream(device.index), *args)
     else:
         with torch.cuda.device(device):
@@ -456,7 +457,7 @@ def checkpoint8_restore(ck, out=None):
         raise ValueError('expected a Checkpoint8')
     C = ck.shape[4] or 1
     if out is None:
-        out, ldc = torch.empty(ck.shape, dtype=ck.dtype, device=ck.device), C
+        out, ldc = torch.empty(*ck.shape, dtype=ck.dtype, device=ck.device), C
     else:
         ldc = _chk_any(out, 'out', ck.shape, ck.dtype, ck.device)
     _call(ck.device, _lib.load().e3_checkpoint8_unpack, _DT[ck.dtype], ck.q.data_ptr(), ck.scale.data_ptr(), ck.q.numel() // C, C, out.data_ptr(), ldc)
@@ -514,7 +515,7 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, activation='
         y, y_ldc = out, _chk_any(out, 'out', shape, dtype, device)
         _chk_out(out, x)
     L = _lib.load()
-    mean = torch.empty((dims[0], num_groups), dtype=torch.float32, device=device)
+    mean = torch.empty(dims[0], num_groups, dtype=torch.float32, device=device)
     rstd = torch.empty_like(mean)
     ck = _new_checkpoint(x) if checkpoint else None
     nbytes = L.e3_group_norm_workspace_bytes(*dims, 0)           # (0 for small groups)
@@ -535,7 +536,7 @@ def group_norm_act_apply(x, mean, rstd, weight=None, bias=None, activation='relu
     C = dims[4]
     weight, bias, wp, bp = _affine(weight, bias, C, device)
     if out is None:
-        y, y_ldc = torch.empty(shape, dtype=dtype, device=device) if src[0] is None else _like(x), C
+        y, y_ldc = torch.empty(*shape, dtype=dtype, device=device) if src[0] is None else _like(x), C
     else:
         y, y_ldc = out, _chk_any(out, 'out', shape, dtype, device)
         if src[0] is not None:
@@ -560,7 +561,7 @@ def group_norm_act_bwd(x, mean, rstd, dy, weight=None, bias=None, activation='re
     dw = torch.empty(C, dtype=torch.float32, device=device)
     db = torch.empty_like(dw)
     nbytes = L.e3_group_norm_workspace_bytes(*dims, 1)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
     _call(device, L.e3_group_norm_act_bwd, _DT[dtype], *src, mean.data_ptr(), rstd.data_ptr(), wp, bp, slope, dy.data_ptr(), dy_ldc, dx.data_ptr(), C,
-          dw.data_ptr(), db.data_ptr(), *dims, ws.data_ptr(), nbytes)
+          dw.data_ptr(), db.data_ptr(), *dims, ws.data_ptr() if nbytes else None, nbytes)
     return dx, dw, db

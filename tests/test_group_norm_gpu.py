@@ -231,6 +231,33 @@ def test_backward(ops, size, dtype):
             within(g, r, e, dtype if name == 'dx' else torch.float32, f'{act} {name}')
 
 
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('size', [
+    (1, 2, 16, 32, 8, 1),          # 8192 elements to a group: the largest that one workgroup takes
+    (1, 1, 25, 41, 8, 1),          # 8200
+    (2, 1, 16, 32, 8, 1),          # 8192 in two samples
+    (2, 1, 19, 27, 8, 1),          # 8208
+    (1, 1, 1, 16, 512, 1),         # the widest bundle
+    (2, 1, 1, 2, 520, 1),          # wider
+    (1, 1, 3, 5, 96, 48),          # groups of 2, 4 channels in pieces of 4 and 8
+    (2, 1, 7, 3, 64, 16),
+    (2, 3, 4, 5, 24, 24),
+    (2, 1, 9, 7, 60, 5),           # groups of 12
+    (1, 1, 64, 63, 1, 1),          # single channels
+])
+def test_backward_of_small_groups(ops, size, dtype):
+    N, D, H, W, C, G = size
+    for act, ldc in (('relu', C), ('silu', C + 8), ('leaky', C + 3)):
+        x, dy, w, b = make(size, dtype, seed=21, ldc=ldc)
+        _, mean, rstd, ck = ops.group_norm_act(x, G, w, b, activation=act, checkpoint=True)
+        val = (ck.q.cpu().float() * ck.scale.cpu().repeat_interleave(64)[:ck.q.numel()]).view(x.shape).cuda()       # (fp32 product: the checkpoint's values)
+        for src, at in ((x, x), (ck, val)):
+            got = ops.group_norm_act_bwd(src, mean, rstd, dy, w, b, activation=act)
+            want, err = ref_bwd(at, mean, rstd, dy, w, b, act)
+            for g, r, e, name in zip(got, want, err, ('dx', 'dweight', 'dbias')):
+                within(g, r, e, dtype if name == 'dx' else torch.float32, f'{act} {name}')
+
+
 def test_backward_against_differences(ops):
     size = (2, 2, 3, 4, 16, 4)
     x, dy, w, b = make(size, torch.float32, seed=3)
