@@ -911,7 +911,8 @@ int e3_group_norm_act_bwd(void* stream, int dtype, const void* x, int x_ldc, con
     E3_REQUIRE(dy && dx && mean && rstd && (x || (q && q_scale)), E3_ERR_INVALID, "null argument");
     E3_REQUIRE((!x || x_ldc >= C) && dy_ldc >= C && dx_ldc >= C, E3_ERR_INVALID, "rows are shorter than the channel count");
     const size_t need = workspace_bytes(sh, true);
-    E3_REQUIRE(workspace_bytes_ >= need && (workspace || !need), E3_ERR_WORKSPACE, "workspace too small");
+    E3_REQUIRE(workspace || !need, E3_ERR_INVALID, "null argument");
+    E3_REQUIRE(workspace_bytes_ >= need, E3_ERR_WORKSPACE, "workspace too small");
     GnArgs a{};
     a.x = x; a.x_ldc = x_ldc; a.q = q; a.qs = q_scale; a.dy = dy; a.dy_ldc = dy_ldc; a.out = dx; a.out_ldc = dx_ldc;
     a.mean = mean; a.rstd = rstd; a.gamma = gamma; a.beta = beta; a.slope = act_slope; a.dgamma = dgamma; a.dbeta = dbeta;
