@@ -11,6 +11,10 @@
 // consecutive channels of a piece that surely share a group (8, 4 or 1): V / UN constants or sums per thread instead of V, which decides the register count.
 //   forward:   statistics (read x) -> apply (read x, write y [, write the checkpoint])
 //   backward:  reduce (read x, dy) -> apply (read x, dy, write dx)
+//   small groups: one launch each way, the pieces held in registers in between
+// What bounds them: HBM, or the memory-side cache, for tensors above some 16 MB, where the second read of the inputs is the price of two passes; below, the latency of
+// two dependent launches (4 - 6 us each), and of the calling program.  2 x 64 x 128 x 128 x 32, 8 groups:
+//   fp32 forward 46 us (5.8 TB/s) + 83 (6.5), fp32 backward from a checkpoint 64 (5.3) + 104 (5.8), bf16 backward 51 (5.3) + 66 (6.1)
 // Sums leave a workgroup as fp64 records [sample][chunk][..], merged in a fixed order: results do not depend on timing.  Every workgroup of the apply pass
 // merges its sample's records itself (a few tens of KB out of L2, about 1 us) instead of waiting for a third launch in between; where the records of a
 // sample are more than MERGE_MAX a finalising launch does it.
@@ -105,13 +109,14 @@ template <typename T, typename F> __device__ __forceinline__ void sum_rows(const
 __device__ __forceinline__ void merge_records(const double* rec, int chunks, int units, int per, double* sh) {
     const int rows = blockDim.x / units, T = rows * units, n = chunks * units;
     double s = 0.0, t = 0.0;
+    constexpr int M = 8;                     // records in flight (4: 0.5 us more for 4096 records)
     if ((int)threadIdx.x < T)
-        for (int j = threadIdx.x; j < n; j += 4 * T) {
-            double2 v[4];
+        for (int j = threadIdx.x; j < n; j += M * T) {
+            double2 v[M];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) { v[k] = make_double2(0.0, 0.0); if (j + k * T < n) v[k] = *reinterpret_cast<const double2*>(rec + 2 * (size_t)(j + k * T)); }
+            for (int k = 0; k < M; ++k) { v[k] = make_double2(0.0, 0.0); if (j + k * T < n) v[k] = *reinterpret_cast<const double2*>(rec + 2 * (size_t)(j + k * T)); }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) { s += v[k].x; t += v[k].y; }
+            for (int k = 0; k < M; ++k) { s += v[k].x; t += v[k].y; }
         }
     double* sums = sh + 2 * blockDim.x;
     if ((int)threadIdx.x < T) { sh[threadIdx.x] = s; sh[T + threadIdx.x] = t; }
@@ -218,7 +223,7 @@ __device__ __forceinline__ void keep_side(const GnArgs& a, int c, const float (&
 }
 
 // ------------------------------------------------------------------------------------------------ forward
-// Sums and sums of squares in fp64: the variance is then a difference that is off by 1e-16 (mean / std)^2 -- less than the inputs' own rounding up to mean / std = 1e5.
+// One read of x: 46 us for 268 MB.  Sums and sums of squares in fp64 (the vector pipes have room: 8 operations per element): the variance is then a difference that is off by 1e-16 (mean / std)^2 -- less than the inputs' own rounding up to mean / std = 1e5.
 template <int V, int UN> struct Moments {
     double s[V / UN], t[V / UN];
     __device__ __forceinline__ Moments() {
@@ -411,7 +416,8 @@ __device__ __forceinline__ void grad_piece(const GnArgs& a, int n, int c, const 
         }
     }
 }
-// Per-thread sums of dz and dz t (h = t rstd: the factor comes last) in fp32 over at most SUM_TERMS elements, everything behind them in fp64.
+// Per-thread sums of dz and dz t (h = t rstd: the factor comes last) in fp32 over at most SUM_TERMS elements, everything behind them in fp64.  The first step is
+// requested in front of the constants (rows of single 16-bit channels, 2.3 M elements: 19.1 -> 16.6 us for the whole backward, others -0.4 ... +0.6).
 template <int DT, int V, int UN, bool CK, bool SILU>
 __global__ __launch_bounds__(MAX_T) void gn_bwd_reduce_kernel(const GnArgs a) {
     extern __shared__ float shf[];
@@ -422,16 +428,20 @@ __global__ __launch_bounds__(MAX_T) void gn_bwd_reduce_kernel(const GnArgs a) {
 #pragma unroll
     for (int e = 0; e < V; ++e) s[e] = t[e] = 0.f;
     if (w.on) {
-        const Consts<V, UN> k = constants<V, UN>(a, a.mean + (size_t)w.n * a.G, a.rstd + (size_t)w.n * a.G, w.c);
-        const float border = border_of<V, UN>(k);
-        for (long long v = w.v0 + w.r; v < w.v1; v += U * a.R) {
-            In<DT, V, CK> in[U]; Raw<DT, V> dy[U];
+        In<DT, V, CK> in[U]; Raw<DT, V> dy[U];
+        auto load = [&](long long v) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 in[u].r = {}; dy[u] = {};
                 const long long row = w.n * a.S + v + u * a.R;
                 if (v + u * a.R < w.v1) { in[u].load(a, row, w.c); dy[u] = load_raw<DT, V>((const T*)a.dy + (size_t)row * a.dy_ldc + w.c); }
             }
+        };
+        long long v = w.v0 + w.r;
+        load(v);                             // (ahead of the constants)
+        const Consts<V, UN> k = constants<V, UN>(a, a.mean + (size_t)w.n * a.G, a.rstd + (size_t)w.n * a.G, w.c);
+        const float border = border_of<V, UN>(k);
+        for (;;) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 float f[V], g[V], dz[V], d[V];
@@ -440,6 +450,9 @@ __global__ __launch_bounds__(MAX_T) void gn_bwd_reduce_kernel(const GnArgs a) {
 #pragma unroll
                 for (int e = 0; e < V; ++e) { s[e] += dz[e]; t[e] = __builtin_fmaf(dz[e], d[e], t[e]); }
             }
+            v += U * a.R;
+            if (v >= w.v1) break;
+            load(v);
         }
 #pragma unroll
         for (int e = 0; e < V; ++e) t[e] *= k.rs[e / UN];
@@ -508,7 +521,7 @@ __global__ __launch_bounds__(256) void gn_bwd_finalize_kernel(const double* __re
     } else sum_channels(part, N * chunks, C, (i - N * G) * 16, dgamma, dbeta, sh);
 }
 
-// dx = a dz - rstd m1 - t rstd^2 m2
+// dx = a dz - rstd m1 - t rstd^2 m2, from the chunk's end to its start; dgamma and dbeta in workgroups of their own in front of the others
 template <int DT, int V, int UN, bool CK, bool SILU>
 __global__ __launch_bounds__(MAX_T) void gn_bwd_apply_kernel(const GnArgs a) {
     extern __shared__ double sh[];
