@@ -32,7 +32,10 @@ template <int DT> __device__ __forceinline__ float to_f32(typename Elem<DT>::T v
 template <int DT> __device__ __forceinline__ typename Elem<DT>::T from_f32(float f) {       // round to nearest even; NaN stays NaN
     if constexpr (DT == DT_F32) return f;
     else if constexpr (DT == DT_BF16) return __builtin_bit_cast(unsigned short, (__bf16)f);
-    else return __builtin_bit_cast(unsigned short, (_Float16)f);
+    else {
+        asm("" : "+v"(f));       // (the fp32 value is the result: hipcc otherwise rounds some forms of its last operation straight to 16 bits, v_fma_mixlo_f16, and forms differ)
+        return __builtin_bit_cast(unsigned short, (_Float16)f);
+    }
 }
 
 // V consecutive channels of a voxel as they lie in memory: a piece of 16 bytes (V = wide_of(type): 4 fp32, 8 16-bit elements; C, row length and address in

@@ -46,10 +46,11 @@ struct GnArgs {
     int N, C, G, cg; long long S;
     int P, PT, tiles, R;                     // pieces per voxel, pieces per tile, tiles, voxels per workgroup step
     int chunks; long long chunk;             // chunks of a sample, voxels of a chunk
-    double* part;                            // records (sum, sum of squares) [N][chunks][C / UN] | (sum dz, sum dz h) [N][chunks][C]
-    double* gpart;                           // backward: (sum gamma dz, sum gamma dz h) [N][chunks][G], or nullptr
+    // records: (sum, sum of squares) [N][chunks][G], or [C / UN] where groups lie across tiles | (sum dz, sum dz h) [N][chunks][C]
+    double* part;
+    double* gpart;                           // backward: (sum gamma dz, sum gamma dz h) [N][chunks][G], or nullptr where groups lie across tiles
     // apply passes that merge the records themselves (rec != nullptr)
-    const double* rec; int rec_chunks, rec_units, rec_per;      // [N][rec_chunks][rec_units] pairs, rec_per units to a group
+    const double* rec; int rec_chunks;       // [N][rec_chunks][G] pairs
     double inv_m; float eps;
     float* mean_out; float* rstd_out;        // forward: the statistics, written by the first workgroup of a sample
     const double* cpart; float* dgamma; float* dbeta; int sum_wgs;      // backward: the first sum_wgs workgroups sum the channel records [N * rec_chunks][C]
@@ -83,9 +84,15 @@ template <int DT, int V, bool NT> struct In<DT, V, true, NT> {
     __device__ __forceinline__ void get(float (&f)[V]) const { unpack_q<V>(r, f); }
 };
 
+// v of the lane that a DPP control names
+template <int CTRL> __device__ __forceinline__ double dpp(double v) {
+    const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, 0xf, 0xf, false), hi = __builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, 0xf, 0xf, false);
+    return __hiloint2double(hi, lo);
+}
+// inside a row of 16 lanes with DPP (pair, quad, half row, row: each step's partner holds the other half's sum), beyond with permutes
 __device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o);
+    v += dpp<0xB1>(v); v += dpp<0x4E>(v); v += dpp<0x141>(v); v += dpp<0x140>(v);
+    v += __shfl_xor(v, 16); v += __shfl_xor(v, 32);
     return v;
 }
 
@@ -104,9 +111,24 @@ template <typename T, typename F> __device__ __forceinline__ void sum_rows(const
     }
 }
 
-// Merges a sample's records [chunks][units] of pairs into sh[2 g], sh[2 g + 1] for its groups (per units each).  Threads read the records in memory order and
-// keep their unit; rows, then units of a group, are added in a fixed order.  sh: 2 blockDim + 2 units doubles at least.
-__device__ __forceinline__ void merge_records(const double* rec, int chunks, int units, int per, double* sh) {
+// Sums of `per` consecutive pairs in LDS for each of `groups` groups, in the same manner
+template <typename F> __device__ __forceinline__ void sum_groups(const double* a, const double* b, int stride, int per, int groups, F done) {
+    int L = 64;
+    while (L > 1 && (groups * L > (int)blockDim.x || L >= 2 * per)) L >>= 1;
+    const int l = threadIdx.x & (L - 1);
+    for (int g0 = 0; g0 < groups; g0 += blockDim.x / L) {
+        const int g = g0 + threadIdx.x / L;
+        double s = 0.0, t = 0.0;
+        if (g < groups)
+            for (int k = l; k < per; k += L) { s += a[(g * per + k) * stride]; t += b[(g * per + k) * stride]; }
+        for (int o = L >> 1; o >= 1; o >>= 1) { s += __shfl_xor(s, o); t += __shfl_xor(t, o); }
+        if (l == 0 && g < groups) done(g, s, t);
+    }
+}
+
+// Merges a sample's records [chunks][units] of pairs, a unit for each group, into sh[2 g], sh[2 g + 1].  Threads read the records in memory order and
+// keep their unit; rows are added in a fixed order.  sh: 2 blockDim + 2 units doubles at least.
+__device__ __forceinline__ void merge_records(const double* rec, int chunks, int units, double* sh) {
     const int rows = blockDim.x / units, T = rows * units, n = chunks * units;
     double s = 0.0, t = 0.0;
     constexpr int M = 8;                     // records in flight (4: 0.5 us more for 4096 records)
@@ -123,14 +145,12 @@ __device__ __forceinline__ void merge_records(const double* rec, int chunks, int
     __syncthreads();
     sum_rows(sh, sh + T, rows, units, [&](int u, double x, double y) { sums[2 * u] = x; sums[2 * u + 1] = y; });
     __syncthreads();
-    for (int g = threadIdx.x; g < units / per; g += blockDim.x) {
-        double x = 0.0, y = 0.0;
-        for (int k = 0; k < per; ++k) { x += sums[2 * (g * per + k)]; y += sums[2 * (g * per + k) + 1]; }
-        sh[2 * g] = x; sh[2 * g + 1] = y;
-    }
+    for (int g = threadIdx.x; g < 2 * units; g += blockDim.x) sh[g] = sums[g];
     __syncthreads();
 }
-constexpr int MERGE_MAX = 4096;              // records of a sample that the apply pass merges itself (64 KB)
+// records of a sample that the apply pass merges itself (128 KB out of L2): at 5376 of them 22.0 us for a backward of 2 x 7 x 82 x 19 x 168 in 21 groups instead of 23.4 with a
+// finaliser's launch in between, which costs the host 4 us more; 16384 (512 chunks of 32 groups) the same as the launch, 42.0 : 40.1 in fp32, 29.3 : 31.2 in fp16
+constexpr int MERGE_MAX = 8192;
 constexpr int MERGE_UNITS = 128;             // ... of at most so many units (a workgroup has 192 threads or more)
 
 __device__ __forceinline__ void statistics_of(double s, double t, double inv_m, float eps, float& mean, float& rstd) {
@@ -258,9 +278,16 @@ __global__ __launch_bounds__(MAX_T) void gn_stats_kernel(const GnArgs a) {
         for (int u = 0; u < K; ++u) { const int i = w.r * units + (int)(threadIdx.x % a.PT) * K + u; sh[i] = m.s[u]; s2[i] = m.t[u]; }
     }
     __syncthreads();
-    const int all = a.C / UN, first = w.tile * units;
-    double* o = a.part + (size_t)(blockIdx.x / a.tiles) * all * 2;
-    sum_rows(sh, s2, a.R, units, [&](int u, double x, double y) { if (first + u < all) { o[(first + u) * 2] = x; o[(first + u) * 2 + 1] = y; } });
+    if (a.tiles > 1) {
+        const int all = a.C / UN, first = w.tile * units;
+        double* o = a.part + (size_t)(blockIdx.x / a.tiles) * all * 2;
+        sum_rows(sh, s2, a.R, units, [&](int u, double x, double y) { if (first + u < all) { o[(first + u) * 2] = x; o[(first + u) * 2 + 1] = y; } });
+    } else {
+        double* o = a.part + (size_t)blockIdx.x * a.G * 2;
+        sum_rows(sh, s2, a.R, units, [&](int u, double x, double y) { sh[u] = x; s2[u] = y; });      // (a unit's column is read by its own lanes only)
+        __syncthreads();
+        sum_groups(sh, s2, 1, a.cg / UN, a.G, [&](int g, double x, double y) { o[2 * g] = x; o[2 * g + 1] = y; });
+    }
 }
 
 // NT: the input is read for the last time and the output written past the caches (non-temporal), which leaves the memory-side cache to what the statistics or
@@ -288,7 +315,7 @@ __global__ __launch_bounds__(MAX_T) void gn_apply_kernel(const GnArgs a) {
     load(vb);
     const float* mean = a.mean + (size_t)w.n * a.G; const float* rstd = a.rstd + (size_t)w.n * a.G;
     if (a.rec) {                             // (uniform)
-        merge_records(a.rec + (size_t)w.n * a.rec_chunks * a.rec_units * 2, a.rec_chunks, a.rec_units, a.rec_per, sh);
+        merge_records(a.rec + (size_t)w.n * a.rec_chunks * a.G * 2, a.rec_chunks, a.G, sh);
         float* st = reinterpret_cast<float*>(sh + 2 * blockDim.x);
         for (int g = threadIdx.x; g < a.G; g += blockDim.x) {
             statistics_of(sh[2 * g], sh[2 * g + 1], a.inv_m, a.eps, st[g], st[a.G + g]);
@@ -475,11 +502,7 @@ __global__ __launch_bounds__(MAX_T) void gn_bwd_reduce_kernel(const GnArgs a) {
     if (a.gpart) {                           // (one tile: all channels of the sample's chunk are here)
         __syncthreads();
         double* p = a.gpart + (size_t)blockIdx.x * a.G * 2;
-        for (int g = threadIdx.x; g < a.G; g += blockDim.x) {
-            double x = 0.0, y = 0.0;
-            for (int e = 0; e < a.cg; ++e) { x += gs[2 * (g * a.cg + e)]; y += gs[2 * (g * a.cg + e) + 1]; }
-            p[2 * g] = x; p[2 * g + 1] = y;
-        }
+        sum_groups(gs, gs + 1, 2, a.cg, a.G, [&](int g, double x, double y) { p[2 * g] = x; p[2 * g + 1] = y; });
     }
 }
 
@@ -502,15 +525,20 @@ __device__ __forceinline__ void sum_channels(const double* part, int records, in
     });
 }
 
-// workgroups [0, N G): m1, m2 of a group; the ones behind them: dgamma, dbeta of 16 channels each
-__global__ __launch_bounds__(256) void gn_bwd_finalize_kernel(const double* __restrict__ part, int N, int chunks, int C, int G, const float* __restrict__ gamma, double inv_m,
+// workgroups [0, N G): m1, m2 of a group, from its records or its channels' ones; the ones behind them: dgamma, dbeta of 16 channels each
+__global__ __launch_bounds__(256) void gn_bwd_finalize_kernel(const double* __restrict__ part, const double* __restrict__ gpart, int N, int chunks, int C, int G, const float* __restrict__ gamma, double inv_m,
                                                               float* __restrict__ m1, float* __restrict__ m2, float* __restrict__ dgamma, float* __restrict__ dbeta) {
     __shared__ double sh[512];
     const int i = blockIdx.x, cg = C / G;
     if (i < N * G) {
         double s = 0.0, t = 0.0;
         const int n = i / G, c0 = (i % G) * cg;
-        for (long long k = threadIdx.x; k < (long long)chunks * cg; k += 256) {
+        if (gpart)
+            for (int k = threadIdx.x; k < chunks; k += 256) {
+                const double* r = gpart + ((size_t)((size_t)n * chunks + k) * G + i % G) * 2;
+                s += r[0]; t += r[1];
+            }
+        else for (long long k = threadIdx.x; k < (long long)chunks * cg; k += 256) {
             const int c = c0 + (int)(k % cg);
             const double* r = part + ((size_t)((size_t)n * chunks + k / cg) * C + c) * 2;
             const double g = gamma ? (double)gamma[c] : 1.0;
@@ -543,7 +571,7 @@ __global__ __launch_bounds__(MAX_T) void gn_bwd_apply_kernel(const GnArgs a) {
     const int step = U * a.R;                // (from the end, as in the forward)
     long long vb = w.v0 + (w.v1 - w.v0 - 1) / step * step;
     load(vb);
-    if (a.rec) merge_records(a.rec + (size_t)w.n * a.rec_chunks * a.rec_units * 2, a.rec_chunks, a.rec_units, a.rec_per, sh);
+    if (a.rec) merge_records(a.rec + (size_t)w.n * a.rec_chunks * a.G * 2, a.rec_chunks, a.G, sh);
     if (!w.on) return;
     const Consts<V, UN> k = constants<V, UN>(a, a.mean + (size_t)w.n * a.G, a.rstd + (size_t)w.n * a.G, w.c);
     const float border = border_of<V, UN>(k);
@@ -685,20 +713,24 @@ template <int V> void map_pass(GnArgs& a, const Shape& sh, int target, int U, bo
 dim3 grid_of(const GnArgs& a) { return dim3((unsigned)((long long)a.N * a.chunks * a.tiles)); }
 dim3 block_of(const GnArgs& a) { return dim3((unsigned)((a.R * a.PT + 63) / 64 * 64)); }
 
-// (UN of the kernels: the statistics' records have C / UN units)
+// UN of the kernels
 int unit_of(int V, int cg) { return V >= 8 && cg % 8 == 0 ? 8 : V >= 4 && cg % 4 == 0 ? 4 : 1; }
 
+// units of a statistics record
+int units_of(const GnArgs& a, int un) { return a.tiles > 1 ? a.C / un : a.G; }
 template <int V> size_t fwd_part_doubles(const Shape& sh) {
     GnArgs a{}; map_pass<V>(a, sh, PASS_WGS, U1<V>, false);
-    return (size_t)sh.N * a.chunks * (sh.C / unit_of(V, sh.C / sh.G)) * 2;
+    return (size_t)sh.N * a.chunks * units_of(a, unit_of(V, a.cg)) * 2;
 }
-// what lies in the workspace of a backward pass: channel records, then group records (`merge`) or m1 and m2
-struct BwdSpace { size_t channels, behind; bool merge; };
+// what lies in the workspace of a backward pass: channel records, group records where a workgroup holds whole groups, and, where no apply pass merges those, m1 and m2
+struct BwdSpace { size_t channels, groups, behind; bool merge; };
 BwdSpace bwd_space(const GnArgs& a, const Shape& sh) {
     BwdSpace b;
-    b.merge = a.tiles == 1 && sh.C <= 1024 && sh.G <= MERGE_UNITS && (long long)a.chunks * sh.G <= MERGE_MAX;
+    const bool whole = a.tiles == 1 && sh.C <= 2048;         // (16 bytes of LDS per channel beside the sums' 32 KB)
+    b.merge = whole && sh.G <= MERGE_UNITS && (long long)a.chunks * sh.G <= MERGE_MAX;
+    b.groups = whole ? align_up((size_t)sh.N * a.chunks * sh.G * 2 * sizeof(double), 256) : 0;
     b.channels = align_up((size_t)sh.N * a.chunks * sh.C * 2 * sizeof(double), 256);
-    b.behind = b.merge ? (size_t)sh.N * a.chunks * sh.G * 2 * sizeof(double) : (size_t)2 * sh.N * sh.G * sizeof(float);
+    b.behind = b.merge ? 0 : (size_t)2 * sh.N * sh.G * sizeof(float);
     return b;
 }
 size_t max2(size_t a, size_t b) { return a > b ? a : b; }
@@ -724,11 +756,11 @@ template <int V> bool map_group_bwd(GnArgs& a, const Shape& sh) {
 template <int V> size_t space_of(const Shape& sh, bool backward) {
     if (sh.C % V != 0) return 0;
     GnArgs a{};
-    if (backward && map_group_bwd<V>(a, sh)) return 0;
-    if (!backward) return map_group<V>(a, sh) ? 0 : fwd_part_doubles<V>(sh) * sizeof(double);
+    if (backward && (map_group_bwd<V>(a, sh) || map_group_bwd<1>(a, sh))) return 0;
+    if (!backward) return map_group<V>(a, sh) || map_group<1>(a, sh) ? 0 : fwd_part_doubles<V>(sh) * sizeof(double);
     map_pass<V>(a, sh, PASS_WGS, U2<V>, false, SUM_TERMS);
     const BwdSpace b = bwd_space(a, sh);
-    return b.channels + b.behind;
+    return b.channels + b.groups + b.behind;
 }
 size_t workspace_bytes(const Shape& sh, bool backward) {      // (for every type and alignment)
     return max2(space_of<1>(sh, backward), max2(space_of<4>(sh, backward), space_of<8>(sh, backward)));
@@ -746,7 +778,7 @@ template <int DT, int V, int UN, bool CK, bool BEHIND> void launch_apply(GnArgs 
     const bool keep = a.q_out != nullptr;
     // (merging the records costs a workgroup 1 - 2 us: twice the workgroups without it, 74 -> 53 us for 2 x 64 x 128 x 128 x 32 in bf16)
     map_pass<V>(a, sh, a.rec ? PASS_WGS : 2 * PASS_WGS, U1<V>, keep);
-    const size_t lds = a.rec ? merge_lds(a, a.rec_units) : 0;
+    const size_t lds = a.rec ? merge_lds(a, sh.G) : 0;
     constexpr bool NT = V > 1 && (BEHIND || CK);
     if constexpr (V > 1 && BEHIND) {
         if (keep) { GN_LAUNCH((gn_apply_kernel<DT, V, UN, CK, SILU, true, NT>), grid_of(a), block_of(a), lds, s, a); return; }
@@ -787,18 +819,21 @@ template <int DT, int V, int UN> int forward(GnArgs a, const Shape& sh, void* ws
         E3_CHECK_HIP(hipGetLastError());
         return rc;
     }
+    if constexpr (V > 1) {                   // (small groups of a channel count that pieces do not fit: element by element)
+        if (map_group<1>(a, sh)) return forward<DT, 1, 1>(a, sh, ws, s);
+    }
     GnArgs st = a;
     map_pass<V>(st, sh, PASS_WGS, U1<V>, false);
     st.part = (double*)ws;
-    const int units = sh.C / UN, per = st.cg / UN;
+    const int units = units_of(st, UN);
     hipLaunchKernelGGL((gn_stats_kernel<DT, V, UN>), grid_of(st), block_of(st), (size_t)st.R * st.PT * (V / UN) * 2 * sizeof(double), s, st);
     a.mean = a.mean_out; a.rstd = a.rstd_out;
     // the checkpoint rides in the apply pass where its blocks are whole there; otherwise it is a pass of its own: behind the apply pass, or, in place, in front of it
     GnArgs m{}; map_pass<V>(m, sh, PASS_WGS, U1<V>, true);
     const bool fused = a.q_out && V > 1 && m.tiles == 1 && m.R * m.PT <= MAX_T && ((unsigned long long)sh.S * sh.C) % CK_BLOCK == 0 && (uintptr_t)a.q_out % V == 0;
     const bool before = a.q_out && !fused && a.out == a.x;
-    if (!before && (long long)st.chunks * units <= MERGE_MAX && units <= MERGE_UNITS) { a.rec = st.part; a.rec_chunks = st.chunks; a.rec_units = units; a.rec_per = per; }
-    else hipLaunchKernelGGL(gn_finalize_kernel, dim3(sh.N * sh.G), dim3(256), 0, s, st.part, st.chunks, units, per, st.inv_m, a.eps, a.mean_out, a.rstd_out);
+    if (!before && st.tiles == 1 && (long long)st.chunks * sh.G <= MERGE_MAX && sh.G <= MERGE_UNITS) { a.rec = st.part; a.rec_chunks = st.chunks; }
+    else hipLaunchKernelGGL(gn_finalize_kernel, dim3(sh.N * sh.G), dim3(256), 0, s, st.part, st.chunks, units, units / sh.G, st.inv_m, a.eps, a.mean_out, a.rstd_out);
     if (before) { const int rc = pack_behind(DT, a, sh, s); if (rc) return rc; }
     GnArgs ap = a;
     if (!fused) ap.q_out = nullptr;
@@ -814,25 +849,27 @@ template <int DT, int V, int UN, bool CK> int backward(GnArgs a, const Shape& sh
         E3_CHECK_HIP(hipGetLastError());
         return E3_OK;
     }
+    if constexpr (V > 1) {
+        if (map_group_bwd<1>(a, sh)) return backward<DT, 1, 1, CK>(a, sh, ws, s);
+    }
     GnArgs st = a;
     map_pass<V>(st, sh, PASS_WGS, U2<V>, false, SUM_TERMS);
     st.part = (double*)ws;
     const BwdSpace space = bwd_space(st, sh);
-    void* behind = (char*)ws + space.channels;
-    if (space.merge) st.gpart = (double*)behind;
-    const size_t lds = align_up((size_t)st.R * st.PT * V * 2 * sizeof(float), 8) + (space.merge ? (size_t)sh.C * 2 * sizeof(double) : 0);
+    if (space.groups) st.gpart = (double*)((char*)ws + space.channels);
+    const size_t lds = align_up((size_t)st.R * st.PT * V * 2 * sizeof(float), 8) + (space.groups ? (size_t)sh.C * 2 * sizeof(double) : 0);
     GN_LAUNCH((gn_bwd_reduce_kernel<DT, V, UN, CK, SILU>), grid_of(st), block_of(st), lds, s, st);
     map_pass<V>(a, sh, PASS_WGS, U2<V>, false);
     size_t alds = 0;
     const int sums = (a.dgamma || a.dbeta) ? (sh.C + 15) / 16 : 0;
     if (space.merge) {
-        a.rec = st.gpart; a.rec_chunks = st.chunks; a.rec_units = sh.G; a.rec_per = 1;
+        a.rec = st.gpart; a.rec_chunks = st.chunks;
         a.cpart = st.part; a.sum_wgs = sums;
         alds = merge_lds(a, sh.G);
     } else {
-        float* m1 = (float*)behind;
+        float* m1 = (float*)((char*)ws + space.channels + space.groups);
         float* m2 = m1 + (size_t)sh.N * sh.G;
-        hipLaunchKernelGGL(gn_bwd_finalize_kernel, dim3(sh.N * sh.G + sums), dim3(256), 0, s, st.part, sh.N, st.chunks, sh.C, sh.G, a.gamma, a.inv_m, m1, m2, a.dgamma, a.dbeta);
+        hipLaunchKernelGGL(gn_bwd_finalize_kernel, dim3(sh.N * sh.G + sums), dim3(256), 0, s, st.part, st.gpart, sh.N, st.chunks, sh.C, sh.G, a.gamma, a.inv_m, m1, m2, a.dgamma, a.dbeta);
         a.m1 = m1; a.m2 = m2;
     }
     const dim3 grid(grid_of(a).x + a.sum_wgs);
