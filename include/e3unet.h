@@ -189,8 +189,9 @@ int e3_unet_backward_loss(e3_unet_plan* plan, void* stream, const float* y, cons
  * for, unet.py:918-935): _keep writes the raw conv outputs of `saved` as 8-bit checkpoints (see e3_checkpoint8_pack) beside the norms' fp32
  * vectors into `kept` (e3_unet_checkpoint8_bytes() bytes, about 1/7 of `saved`), after which `saved` may be reused; _restore fills a `saved`
  * buffer for e3_unet_backward* of the same plan, shape and parameters, recomputing the activations from the restored tensors.  The gradients are
- * those of the rounded tensors; the rounding keeps every element on its side of a ReLU's border and every pooling window's maximum in place.  nn.RReLU: e3_unet_set_rrelu with the forward's seed first.  fp32 path; 'same' convs, transposed convs and a
- * norm behind every conv, no attention, not the ResUNet (E3_ERR_UNSUPPORTED otherwise). */
+ * those of the rounded tensors; the rounding keeps every element on its side of a ReLU's border and every pooling window's maximum in place.
+ * nn.RReLU: e3_unet_set_rrelu with the forward's seed first.  fp32 path; 'same' convs, transposed convs and a norm behind every conv, no attention,
+ * not the ResUNet (E3_ERR_UNSUPPORTED otherwise). */
 int e3_unet_checkpoint8_bytes(const e3_unet_plan* plan, int N, int D, int H, int W, size_t* kept_bytes);
 int e3_unet_checkpoint8_keep(const e3_unet_plan* plan, void* stream, int N, int D, int H, int W, void* const* params,
                              const void* saved, size_t saved_bytes, void* kept, size_t kept_bytes);
@@ -284,7 +285,8 @@ int e3_bn_relu_bwd(void* stream, const float* x, int x_ldc, const float* mean, c
  *   mean, rstd:  [N][G] fp32 outputs (inputs of _apply and _bwd).
  *   q, q_scale:  NULL, or the 8-bit checkpoint of x that the same call writes (see e3_checkpoint8_pack; N*D*H*W*C codes).
  *   workspace:   e3_group_norm_workspace_bytes(.., backward) bytes; NULL where that is 0 (small groups need none).
- * y may be x itself (the same view), dx may be dy.  Statistics and sums are fp32 values of fp64 sums in a fixed order. */
+ * y may be x itself (the same view), dx may be dy.  Statistics are fp32 values of fp64 sums; gradient sums add at most 512 elements in fp32, then in fp64; the
+ * order is fixed, two identical calls give the same bits.  At most 2^23 - 1 groups in all samples and 2^26 channels (E3_ERR_UNSUPPORTED). */
 size_t e3_group_norm_workspace_bytes(int N, int D, int H, int W, int C, int G, int backward);
 int e3_group_norm_act_fwd(void* stream, int dtype, const void* x, int x_ldc, const float* gamma, const float* beta, float eps, float act_slope,
                           void* y, int y_ldc, float* mean, float* rstd, signed char* q, float* q_scale,
