@@ -926,6 +926,7 @@ int e3_group_norm_act_fwd(void* stream, int dtype, const void* x, int x_ldc, con
     E3_REQUIRE(eps >= 0.f, E3_ERR_INVALID, "eps must not be negative");
     const size_t need = workspace_bytes(sh, false);
     E3_REQUIRE(workspace_bytes_ >= need && (workspace || !need), E3_ERR_WORKSPACE, "workspace too small");
+    E3_REQUIRE(aligned16(workspace), E3_ERR_INVALID, "the workspace must be aligned to 16 bytes");
     GnArgs a{};
     a.x = x; a.x_ldc = x_ldc; a.out = y; a.out_ldc = y_ldc; a.gamma = gamma; a.beta = beta; a.slope = act_slope; a.q_out = q; a.qs_out = q_scale;
     a.eps = eps; a.mean_out = mean; a.rstd_out = rstd;
@@ -963,6 +964,7 @@ int e3_group_norm_act_bwd(void* stream, int dtype, const void* x, int x_ldc, con
     const size_t need = workspace_bytes(sh, true);
     E3_REQUIRE(workspace || !need, E3_ERR_INVALID, "null argument");
     E3_REQUIRE(workspace_bytes_ >= need, E3_ERR_WORKSPACE, "workspace too small");
+    E3_REQUIRE(aligned16(workspace), E3_ERR_INVALID, "the workspace must be aligned to 16 bytes");
     GnArgs a{};
     a.x = x; a.x_ldc = x_ldc; a.q = q; a.qs = q_scale; a.dy = dy; a.dy_ldc = dy_ldc; a.out = dx; a.out_ldc = dx_ldc;
     a.mean = mean; a.rstd = rstd; a.gamma = gamma; a.beta = beta; a.slope = act_slope; a.dgamma = dgamma; a.dbeta = dbeta;

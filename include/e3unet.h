@@ -284,7 +284,7 @@ int e3_bn_relu_bwd(void* stream, const float* x, int x_ldc, const float* mean, c
  *   gamma, beta: [C] fp32, or NULL (1 and 0).  act_slope: 0 = ReLU, (0, 1) = LeakyReLU, 1 = identity, 2 = SiLU.
  *   mean, rstd:  [N][G] fp32 outputs (inputs of _apply and _bwd).
  *   q, q_scale:  NULL, or the 8-bit checkpoint of x that the same call writes (see e3_checkpoint8_pack; N*D*H*W*C codes).
- *   workspace:   e3_group_norm_workspace_bytes(.., backward) bytes; NULL where that is 0 (small groups need none).
+ *   workspace:   e3_group_norm_workspace_bytes(.., backward) bytes, 16-byte aligned; NULL where that is 0 (small groups need none).
  * y may be x itself (the same view), dx may be dy.  Statistics are fp32 values of fp64 sums; gradient sums add at most 512 elements in fp32, then in fp64; the
  * order is fixed, two identical calls give the same bits.  At most 2^23 - 1 groups in all samples and 2^26 channels (E3_ERR_UNSUPPORTED). */
 size_t e3_group_norm_workspace_bytes(int N, int D, int H, int W, int C, int G, int backward);

@@ -184,6 +184,30 @@ def test_views(ops, dtype, C, G, ldc):
     torch.testing.assert_close(yin, y, rtol=2 * HALF[dtype] + 2e-6, atol=1e-5)
 
 
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('size', [(2, 5, 9, 13, 32, 4), (1, 3, 4, 5, 16, 2)])
+def test_addresses_that_are_no_multiple_of_16(ops, size, dtype):
+    """Every tensor one element, every checkpoint three codes behind such an address: the results of aligned copies, up to the order of their sums."""
+    C, G = size[4:]
+    x, dy, w, b = make(size, dtype, seed=31)
+    off = lambda t: torch.cat([t.new_zeros(1), t.reshape(-1)])[1:].view(t.shape)       # noqa: E731
+    x1, dy1, y1 = off(x), off(dy), off(torch.zeros_like(x))
+    assert x1.data_ptr() % 16 and x1.is_contiguous()
+    y, mean, rstd, ck = ops.group_norm_act(x, G, w, b, checkpoint=True)
+    _, mean1, rstd1, ck1 = ops.group_norm_act(x1, G, off(w), off(b), checkpoint=True, out=y1)
+    torch.testing.assert_close(mean1, mean, rtol=2 ** -22, atol=1e-7)
+    torch.testing.assert_close(rstd1, rstd, rtol=2 ** -22, atol=0)
+    torch.testing.assert_close(y1, y, rtol=2 * HALF[dtype] + 2e-6, atol=1e-5)
+    assert torch.equal(ck1.scale, ck.scale)
+    q3 = torch.cat([ck.q.new_zeros(3), ck.q])[3:]
+    ck3 = ops.Checkpoint8(q3, off(ck.scale), x.shape, dtype)
+    assert torch.equal(ops.checkpoint8_restore(ck3, out=off(torch.zeros_like(x))), ops.checkpoint8_restore(ck))
+    torch.testing.assert_close(ops.group_norm_act_apply(ck3, mean, rstd, w, b), ops.group_norm_act_apply(ck, mean, rstd, w, b), rtol=2 * HALF[dtype] + 2e-6, atol=1e-6)
+    for src, at in ((x1, x), (ck3, ck)):
+        for g, r in zip(ops.group_norm_act_bwd(src, off(mean), off(rstd), dy1, w, b), ops.group_norm_act_bwd(at, mean, rstd, dy, w, b)):
+            torch.testing.assert_close(g, r, rtol=2e-5 if g.dtype == torch.float32 else 2 * HALF[dtype] + 2e-5, atol=1e-5)
+
+
 def test_large_offset(ops):
     """mean / std = 3000: a variance from fp32 sums of squares would be noise."""
     x, dy, w, b = make((2, 6, 12, 10, 16, 2), torch.float32)

@@ -113,6 +113,16 @@ def test_workspace_sizes(dims):
     assert call('e3_group_norm_workspace_bytes', 1, 4, 8, 8, 128, 8, 0) == 0 < call('e3_group_norm_workspace_bytes', 1, 64, 64, 64, 128, 8, 0)
 
 
+def test_workspaces_off_their_alignment():
+    odd = ctypes.c_void_p((1 << 20) + 8)
+    for backward, name, args in ((0, 'fwd', (None, 0, FAKE, 32, None, None, 1e-5, 0.0, FAKE, 32, FAKE, FAKE, None, None)),
+                                 (1, 'bwd', (None, 0, FAKE, 32, None, None, FAKE, FAKE, None, None, 0.0, FAKE, 32, FAKE, 32, FAKE, FAKE))):
+        dims = (3, 64, 64, 64, 32, 8)
+        need = call('e3_group_norm_workspace_bytes', *dims, backward)
+        assert need > 0 and call(f'e3_group_norm_act_{name}', *args, *dims, odd, ctypes.c_size_t(need)) == 1
+        assert b'aligned' in _lib.load().e3_last_error()
+
+
 def test_sums_of_long_samples_are_cut():
     """A thread's fp32 sums of the backward have at most 512 terms: 256 threads to a workgroup, one (sum, sum) record of doubles per workgroup and channel."""
     voxels = 16384 * 16384
