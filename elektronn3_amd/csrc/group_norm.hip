@@ -14,7 +14,7 @@
 //   small groups: one launch each way, the pieces held in registers in between
 // What bounds them: HBM, or the memory-side cache, for tensors above some 16 MB, where the second read of the inputs is the price of two passes; below, the latency of
 // two dependent launches (4 - 6 us each), and of the calling program.  2 x 64 x 128 x 128 x 32, 8 groups:
-//   fp32 forward 46 us (5.8 TB/s) + 83 (6.5), fp32 backward from a checkpoint 64 (5.3) + 104 (5.8), bf16 backward 51 (5.3) + 66 (6.1)
+//   fp32 forward 46 us (5.8 TB/s) + 83 (6.5), fp32 backward from a checkpoint 64 (5.3) + 97 (6.3), bf16 backward 51 (5.3) + 66 (6.1)
 // Sums leave a workgroup as fp64 records [sample][chunk][..], merged in a fixed order: results do not depend on timing.  Every workgroup of the apply pass
 // merges its sample's records itself (a few tens of KB out of L2, about 1 us) instead of waiting for a third launch in between; where the records of a
 // sample are more than MERGE_MAX a finalising launch does it.
@@ -688,6 +688,15 @@ constexpr int SUM_TERMS = 512;               // fp32 terms of a sum: their round
 
 void set_shape(GnArgs& a, const Shape& sh) { a.N = sh.N; a.S = sh.S; a.C = sh.C; a.G = sh.G; a.cg = sh.C / sh.G; a.inv_m = 1.0 / ((double)sh.S * a.cg); }
 
+// Twice as many where a backward's workgroups have 16 steps or more and a sample's records stay few (2 x 64 x 128 x 128 x 32 in 8 groups: fp32 226 -> 213 us, from a checkpoint 182 -> 167,
+// bf16 from a checkpoint 120 -> 111, but not bf16 116 -> 122; one sample of half the size in 32 groups would lose 65 -> 73), or for rows of single elements, whose loads are small
+// (1 x 19 x 27 x 89 x 65: forward 24 -> 20 us; three workgroups per CU in its backward, from a checkpoint 26 -> 22)
+template <int V> int workgroups(const Shape& sh, bool backward, bool ck = true) {
+    const long long steps = sh.N * sh.S * (sh.C / V) / (PASS_T * U2<V>);
+    if (V == 1) return !backward ? 2 * PASS_WGS : steps >= 2 * PASS_WGS ? PASS_WGS * 3 / 2 : PASS_WGS;
+    return backward && (ck || V < 8) && steps >= 16 * PASS_WGS && 2ll * PASS_WGS * sh.G <= 4096ll * sh.N ? 2 * PASS_WGS : PASS_WGS;
+}
+
 // mapping of a pass; `target`: workgroups that it asks for (at least one per sample and tile); `terms`: voxels of a thread at most, or 0
 template <int V> void map_pass(GnArgs& a, const Shape& sh, int target, int U, bool keep, int terms = 0) {
     set_shape(a, sh);
@@ -719,7 +728,7 @@ int unit_of(int V, int cg) { return V >= 8 && cg % 8 == 0 ? 8 : V >= 4 && cg % 4
 // units of a statistics record
 int units_of(const GnArgs& a, int un) { return a.tiles > 1 ? a.C / un : a.G; }
 template <int V> size_t fwd_part_doubles(const Shape& sh) {
-    GnArgs a{}; map_pass<V>(a, sh, PASS_WGS, U1<V>, false);
+    GnArgs a{}; map_pass<V>(a, sh, workgroups<V>(sh, false), U1<V>, false);
     return (size_t)sh.N * a.chunks * units_of(a, unit_of(V, a.cg)) * 2;
 }
 // what lies in the workspace of a backward pass: channel records, group records where a workgroup holds whole groups, and, where no apply pass merges those, m1 and m2
@@ -758,7 +767,7 @@ template <int V> size_t space_of(const Shape& sh, bool backward) {
     GnArgs a{};
     if (backward && (map_group_bwd<V>(a, sh) || map_group_bwd<1>(a, sh))) return 0;
     if (!backward) return map_group<V>(a, sh) || map_group<1>(a, sh) ? 0 : fwd_part_doubles<V>(sh) * sizeof(double);
-    map_pass<V>(a, sh, PASS_WGS, U2<V>, false, SUM_TERMS);
+    map_pass<V>(a, sh, workgroups<V>(sh, true), U2<V>, false, SUM_TERMS);        // (the most that a backward takes)
     const BwdSpace b = bwd_space(a, sh);
     return b.channels + b.groups + b.behind;
 }
@@ -777,7 +786,7 @@ size_t merge_lds(const GnArgs& a, int units) { return (size_t)2 * (block_of(a).x
 template <int DT, int V, int UN, bool CK, bool BEHIND> void launch_apply(GnArgs a, const Shape& sh, hipStream_t s) {
     const bool keep = a.q_out != nullptr;
     // (merging the records costs a workgroup 1 - 2 us: twice the workgroups without it, 74 -> 53 us for 2 x 64 x 128 x 128 x 32 in bf16)
-    map_pass<V>(a, sh, a.rec ? PASS_WGS : 2 * PASS_WGS, U1<V>, keep);
+    map_pass<V>(a, sh, a.rec ? workgroups<V>(sh, false) : 2 * PASS_WGS, U1<V>, keep);
     const size_t lds = a.rec ? merge_lds(a, sh.G) : 0;
     constexpr bool NT = V > 1 && (BEHIND || CK);
     if constexpr (V > 1 && BEHIND) {
@@ -823,13 +832,13 @@ template <int DT, int V, int UN> int forward(GnArgs a, const Shape& sh, void* ws
         if (map_group<1>(a, sh)) return forward<DT, 1, 1>(a, sh, ws, s);
     }
     GnArgs st = a;
-    map_pass<V>(st, sh, PASS_WGS, U1<V>, false);
+    map_pass<V>(st, sh, workgroups<V>(sh, false), U1<V>, false);
     st.part = (double*)ws;
     const int units = units_of(st, UN);
     hipLaunchKernelGGL((gn_stats_kernel<DT, V, UN>), grid_of(st), block_of(st), (size_t)st.R * st.PT * (V / UN) * 2 * sizeof(double), s, st);
     a.mean = a.mean_out; a.rstd = a.rstd_out;
     // the checkpoint rides in the apply pass where its blocks are whole there; otherwise it is a pass of its own: behind the apply pass, or, in place, in front of it
-    GnArgs m{}; map_pass<V>(m, sh, PASS_WGS, U1<V>, true);
+    GnArgs m{}; map_pass<V>(m, sh, workgroups<V>(sh, false), U1<V>, true);
     const bool fused = a.q_out && V > 1 && m.tiles == 1 && m.R * m.PT <= MAX_T && ((unsigned long long)sh.S * sh.C) % CK_BLOCK == 0 && (uintptr_t)a.q_out % V == 0;
     const bool before = a.q_out && !fused && a.out == a.x;
     if (!before && st.tiles == 1 && (long long)st.chunks * sh.G <= MERGE_MAX && sh.G <= MERGE_UNITS) { a.rec = st.part; a.rec_chunks = st.chunks; }
@@ -853,13 +862,13 @@ template <int DT, int V, int UN, bool CK> int backward(GnArgs a, const Shape& sh
         if (map_group_bwd<1>(a, sh)) return backward<DT, 1, 1, CK>(a, sh, ws, s);
     }
     GnArgs st = a;
-    map_pass<V>(st, sh, PASS_WGS, U2<V>, false, SUM_TERMS);
+    map_pass<V>(st, sh, workgroups<V>(sh, true, CK), U2<V>, false, SUM_TERMS);
     st.part = (double*)ws;
     const BwdSpace space = bwd_space(st, sh);
     if (space.groups) st.gpart = (double*)((char*)ws + space.channels);
     const size_t lds = align_up((size_t)st.R * st.PT * V * 2 * sizeof(float), 8) + (space.groups ? (size_t)sh.C * 2 * sizeof(double) : 0);
     GN_LAUNCH((gn_bwd_reduce_kernel<DT, V, UN, CK, SILU>), grid_of(st), block_of(st), lds, s, st);
-    map_pass<V>(a, sh, PASS_WGS, U2<V>, false);
+    map_pass<V>(a, sh, workgroups<V>(sh, true, CK), U2<V>, false);
     size_t alds = 0;
     const int sums = (a.dgamma || a.dbeta) ? (sh.C + 15) / 16 : 0;
     if (space.merge) {
