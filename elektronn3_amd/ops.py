@@ -30,6 +30,11 @@ def _ldc(t):
         and (N == 1 or sN == D * H * W * ldc or (D == 1 and H == 1 and W == 1))
     if not ok:
         raise ValueError(f'not an NDHWC view: shape {tuple(t.shape)} strides {t.stride()}')
+    return _rows(ldc)
+
+
+def _rows(ldc):
+    """A row length that fits the C ABI's int (ctypes cuts a longer one to 32 bits without an error)."""
     if ldc >= 1 << 31:
         raise ValueError(f'rows of {ldc} elements: longer than the kernels address')
     return ldc
@@ -360,7 +365,9 @@ def _chk_any(t, name, shape=None, dtype=None, device=None):
         raise ValueError(f'{name}: expected shape {tuple(shape)}, {dtype} on {device}, got {tuple(t.shape)}, {t.dtype} on {t.device}')
     if t.dim() != 5:
         raise ValueError(f'{name}: expected a 5D (N, D, H, W, C) tensor, got {t.dim()}D')
-    return t.shape[4] or 1 if t.is_contiguous() else _ldc(t)
+    if not t.is_contiguous():
+        return _ldc(t)
+    return _rows(t.shape[4] or 1)
 
 
 def _span(t):
@@ -415,6 +422,7 @@ class Checkpoint8:
             raise ValueError(f'Checkpoint8: q: expected {n} contiguous int8 codes')
         if scale.dtype != torch.float32 or scale.numel() != -(-n // 64) or not scale.is_contiguous() or scale.device != q.device:
             raise ValueError(f'Checkpoint8: scale: expected {-(-n // 64)} contiguous float32 values on {q.device}')
+        _rows(shape[4])
         if not q.is_cuda:
             raise ValueError('Checkpoint8: expected CUDA tensors (the HIP path has no CPU fallback)')
         self.q, self.scale, self.shape, self.dtype, self.device = q, scale, shape, dtype, q.device
@@ -476,6 +484,8 @@ def _gn_dims(shape, num_groups):
     N, D, H, W, C = shape
     if N < 1 or D < 1 or H < 1 or W < 1 or C < 1:
         raise ValueError(f'x: expected at least one element, got shape {tuple(shape)}')
+    if (N | D | H | W | C) >> 31:                # (ctypes cuts longer ones to 32 bits without an error)
+        raise ValueError(f'x: expected axes below 2^31, got shape {tuple(shape)}')
     if num_groups < 1 or C % num_groups != 0:
         raise ValueError('num_channels must be divisible by num_groups')
     return N, D, H, W, C, num_groups
