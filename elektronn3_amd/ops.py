@@ -377,7 +377,7 @@ def _span(t):
 
 def _chk_out(out, t, name='out'):
     """`out` may be the input itself (the same view); a view that overlaps it otherwise would be read after it was written."""
-    if out.numel() == 0 or (t.data_ptr() == out.data_ptr() and t.stride() == out.stride()):
+    if out.numel() == 0 or (t.data_ptr() == out.data_ptr() and (t.stride() == out.stride() or _ldc(t) == _ldc(out))):      # (axes of one element may have any stride)
         return
     (a, b), (c, d) = _span(t), _span(out)
     if a < d and c < b:
