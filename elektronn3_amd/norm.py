@@ -73,7 +73,8 @@ class GroupNormAct(nn.GroupNorm):
             raise ValueError(f'expected {self.num_channels} channels, got {x.shape[1]}')
         if not x.is_cuda:
             raise RuntimeError('elektronn3_amd.GroupNormAct runs only on a ROCm GPU (hand-written HIP kernels); there is no CPU fallback')
-        return _GroupNormActFunction.apply(x, self.weight, self.bias, self.num_groups, self.eps, self.activation, self.checkpoint and torch.is_grad_enabled())
+        keep = self.checkpoint and torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, self.weight, self.bias))
+        return _GroupNormActFunction.apply(x, self.weight, self.bias, self.num_groups, self.eps, self.activation, keep)
 
     def extra_repr(self):
         return super().extra_repr() + f', activation={self.activation!r}, checkpoint={self.checkpoint}'
