@@ -757,6 +757,21 @@ template <int V> bool map_group(GnArgs& a, const Shape& sh) {
         if (t / a.PT > 0 && sh.S <= t / a.PT) a.R = t / a.PT;
     return true;
 }
+// ... of the forward, for elements of `size` bytes.  A bundle narrower than a 128-byte line moves every line once per bundle in it, to as many workgroups on other XCDs: what that moves is
+// limited.  us for two launches : one, 16-bit types unless said, by megabytes moved so:
+//   pieces: 32: 14.3 : 12.8 (2 x 2048 voxels x 512 in 64 groups), 11.7 : 11.7 (16 x 2048 x 64 in 8), fp32 12.5 : 13.6 (4 x 4096 x 64 in 16); 40: 15.0 : 13.9 (5 x 2048 x 256 in 32);
+//     48: 13.4 : 16.6 (24 x 2048 x 64 in 8); 64: 17.5 : 19.6 (4 x 2048 x 512 in 64); 1024: 76 : 236 (64 of these)
+//   single elements instead of two launches with pieces: 16: 10.7 : 9.1 (2 x 4096 x 32 in 32); 21: 14.6 : 11.9 (16 x 105 x 1200 in 100); 31: 15.0 : 16.6 (300 x 105 x 96 in 8);
+//     32: 11.2 : 10.7, with a checkpoint 13.0 : 17.5 (1 x 4096 x 64 in 64); 41: 15.8 : 21.4 (32 x 105 x 1200 in 100); 1024: 34 : 88 (8 x 4096 x 256 in 256)
+//   single elements in either form: 5 bundles to a line 385: 130 : 113 (400 x 315 x 300 in 25); 21 and 33 of them 41: 15.0 : 10.9 (16 x 315 x 201 in 67), 12.6 : 12.2 (64 x 315 x 33 in 33),
+//     165: 26 : 31, 18 : 33 (four times these)
+// Bundles of whole lines have no limit (1024 x 256 x 512 in 8: 150 : 142).
+template <int V> bool map_group_fwd(GnArgs& a, const Shape& sh, int size, bool rows_of_pieces) {
+    if (!map_group<V>(a, sh)) return false;
+    const long long row = (long long)sh.C * size, width = (long long)a.PT * V * size, line = row < 128 ? row : 128;
+    if (width >= line || (!rows_of_pieces && line <= 8 * width)) return true;
+    return sh.N * sh.S * (row / width) * line <= (V > 1 ? 40ll : rows_of_pieces ? 24ll : 96ll) << 20;
+}
 // ... and of the backward, whose workgroups walk the samples: 6 us for the first and 3 - 9 for each other one (a workgroup's 16-byte pieces lie C elements apart) against
 // 9 - 13 for two launches, which cost the host 5 us more.  1 x 4 x 8 x 8 x 128 in 8 groups, fp16: 8.4 us instead of 12.2, eagerly 13 instead of 18; two samples of it 14.2
 // instead of 12.3, eagerly 14 instead of 18; four 25.8; 16384 elements to a group 15.4 instead of 14.0
@@ -764,11 +779,22 @@ constexpr int GROUP_SAMPLES = 2, GROUP_ELEMS = 8192, GROUP_CHANNELS = 512;      
 template <int V> bool map_group_bwd(GnArgs& a, const Shape& sh) {
     return sh.N <= GROUP_SAMPLES && map_group<V>(a, sh) && a.PT * V <= GROUP_CHANNELS && sh.N * sh.S * a.cg <= GROUP_ELEMS;
 }
+// single elements instead of two launches with pieces: where groups cut the pieces, or (one-channel groups of more voxels than pieces can hold) for one sample: 1 x 4096 voxels x 8, 16, 32,
+// 64, 256 channels in 16 bits 7.2, 10.4, 11.5, 14.4, 21.7 us against 10.5, 10.9, 11.0, 13.6, 23.3 for two launches, but two samples x 16, 64 channels 18.0, 26.3 against 11.0, 13.9
+template <int V> bool map_single_bwd(GnArgs& a, const Shape& sh) {
+    const int cg = sh.C / sh.G;
+    return (sh.N == 1 || (cg % V != 0 && V % cg != 0)) && map_group_bwd<1>(a, sh);
+}
 template <int V> size_t space_of(const Shape& sh, bool backward) {
     if (sh.C % V != 0) return 0;
     GnArgs a{};
-    if (backward && (map_group_bwd<V>(a, sh) || map_group_bwd<1>(a, sh))) return 0;
-    if (!backward) return map_group<V>(a, sh) || map_group<1>(a, sh) ? 0 : fwd_part_doubles<V>(sh) * sizeof(double);
+    if (backward && (map_group_bwd<V>(a, sh) || (V > 1 && map_single_bwd<V>(a, sh)))) return 0;
+    if (!backward) {
+        const int size = V == 8 ? 2 : 4;
+        const bool one = V > 1 ? map_group_fwd<V>(a, sh, size, true) || map_group_fwd<1>(a, sh, size, true)
+                               : map_group_fwd<1>(a, sh, 2, false) && map_group_fwd<1>(a, sh, 4, false);       // (single elements: of every type)
+        return one ? 0 : fwd_part_doubles<V>(sh) * sizeof(double);
+    }
     map_pass<V>(a, sh, workgroups<V>(sh, true), U2<V>, false, SUM_TERMS);        // (the most that a backward takes)
     const BwdSpace b = bwd_space(a, sh);
     return b.channels + b.groups + b.behind;
@@ -825,14 +851,16 @@ template <int DT, int V, int UN> int forward_group(GnArgs a, const Shape& sh, hi
 }
 
 template <int DT, int V, int UN> int forward(GnArgs a, const Shape& sh, void* ws, hipStream_t s) {
-    if (map_group<V>(a, sh)) {
+    constexpr int size = sizeof(typename Elem<DT>::T);
+    if (map_group_fwd<V>(a, sh, size, V > 1)) {
         const int rc = forward_group<DT, V, UN>(a, sh, s);
         E3_CHECK_HIP(hipGetLastError());
         return rc;
     }
-    if constexpr (V > 1) {                   // (small groups of a channel count that pieces do not fit: element by element)
-        if (map_group<1>(a, sh)) return forward<DT, 1, 1>(a, sh, ws, s);
+    if constexpr (V > 1) {                   // (groups that cut the pieces, or one-channel groups of more voxels than pieces can hold: element by element)
+        if (map_group_fwd<1>(a, sh, size, true)) return forward<DT, 1, 1>(a, sh, ws, s);
     }
+    E3_REQUIRE(ws, E3_ERR_WORKSPACE, "workspace too small");         // (where workspace_bytes() and this dispatch disagree)
     GnArgs st = a;
     map_pass<V>(st, sh, workgroups<V>(sh, false), U1<V>, false);
     st.part = (double*)ws;
@@ -861,8 +889,9 @@ template <int DT, int V, int UN, bool CK> int backward(GnArgs a, const Shape& sh
         return E3_OK;
     }
     if constexpr (V > 1) {
-        if (map_group_bwd<1>(a, sh)) return backward<DT, 1, 1, CK>(a, sh, ws, s);
+        if (map_single_bwd<V>(a, sh)) return backward<DT, 1, 1, CK>(a, sh, ws, s);
     }
+    E3_REQUIRE(ws, E3_ERR_WORKSPACE, "workspace too small");
     GnArgs st = a;
     map_pass<V>(st, sh, workgroups<V>(sh, true, CK), U2<V>, false, SUM_TERMS);
     st.part = (double*)ws;
