@@ -1271,7 +1271,8 @@ class UNet(nn.Module):
         ``normalization='group'`` / ``'instance'``, whose batch is one graph per sample.  The outputs are unchanged; the gradients are those of the rounded
         tensors: of every norm's input, an element is off by at most 1/254 of the largest of its block of 64 (:class:`elektronn3_amd.ops.Checkpoint8`),
         and the activations are recomputed from them.  What the reference's ``forward_gradcp`` (unet.py:918-935) trades recomputation for, this trades
-        precision for.  The rounding keeps every element on its side of a ReLU's border and every pooling window's maximum in place.  fp32 compute; transposed
+        precision for.  The rounding keeps elements on their side of a ReLU's border, and a pooling window's maximum in place where a neighbouring code on that
+        side allows it (all but some 10 windows in a million).  fp32 compute; transposed
         up-convolutions, 'same' convolutions and a norm behind every convolution, no attention (NotImplementedError otherwise).  Scripted modules keep
         their activations as they are.  Returns the module."""
         if enabled:

@@ -189,7 +189,8 @@ int e3_unet_backward_loss(e3_unet_plan* plan, void* stream, const float* y, cons
  * for, unet.py:918-935): _keep writes the raw conv outputs of `saved` as 8-bit checkpoints (see e3_checkpoint8_pack) beside the norms' fp32
  * vectors into `kept` (e3_unet_checkpoint8_bytes() bytes, about 1/7 of `saved`), after which `saved` may be reused; _restore fills a `saved`
  * buffer for e3_unet_backward* of the same plan, shape and parameters, recomputing the activations from the restored tensors.  The gradients are
- * those of the rounded tensors; the rounding keeps every element on its side of a ReLU's border and every pooling window's maximum in place.
+ * those of the rounded tensors; the rounding keeps elements on their side of a ReLU's border, and a pooling window's maximum in place where a neighbouring
+ * code on that side allows it (all but some 10 windows in a million).
  * nn.RReLU: e3_unet_set_rrelu with the forward's seed first.  fp32 path; 'same' convs, transposed convs and a norm behind every conv, no attention,
  * not the ResUNet (E3_ERR_UNSUPPORTED otherwise). */
 int e3_unet_checkpoint8_bytes(const e3_unet_plan* plan, int N, int D, int H, int W, size_t* kept_bytes);
