@@ -9,7 +9,8 @@
 //
 // A checkpoint of the input of a norm with ReLU / LeakyReLU is rounded TO ITS SIDE: where x and its rounded value lie on different sides of the activation's border
 // (z = 0), the code is the other neighbour of x, which lies on x's side.  The error there is up to a whole step, but the backward then takes exactly the forward's
-// branch everywhere.  Rounded to nearest, 1 element in 400 of a Gaussian changes sides, and each contributes its whole gradient: 7 % of a layer's gradient norm.
+// branch.  (Not where x is its block's largest and the border lies between it and 127 scale, a rounding apart: the neighbour of +-127 beyond it is no code.)
+// Rounded to nearest, 1 element in 400 of a Gaussian changes sides, and each contributes its whole gradient: 7 % of a layer's gradient norm.
 #pragma once
 #include "common.h"
 

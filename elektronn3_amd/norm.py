@@ -57,7 +57,7 @@ class GroupNormAct(nn.GroupNorm):
 
     ``checkpoint=True`` keeps the input for the backward as an 8-bit checkpoint (:class:`elektronn3_amd.ops.Checkpoint8`, 1.06 bytes per element)
     instead of the tensor: the outputs are the same, the gradients are those of the rounded input (an element is off by at most 1/254 of the largest of its
-    block of 64).  A parameter that is missing (``affine=False``) is 1 or 0.
+    block of 64; with ReLU or LeakyReLU by up to 1/127 next to the activation's border, whose side it keeps).  A parameter that is missing (``affine=False``) is 1 or 0.
 
     ``activation``: ``'relu'``, ``'leaky'``, ``'lin'``, ``'silu'`` or a module of those types (as in ``UNet(activation=...)``)."""
 

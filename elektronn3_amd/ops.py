@@ -409,7 +409,8 @@ def _act_slope(activation):
 class Checkpoint8:
     """An (N, D, H, W, C) activation kept in 8 bits: ``q`` (int8, one code per element in packed NDHWC order) and ``scale`` (float32, one per 64
     elements).  It stands for ``q * scale`` (3.76 times smaller than float32, 1.88 times than a 16-bit type); an element is off by at most half
-    a step, ``amax / 254`` of its block's largest magnitude.  A block with a NaN or an infinity stands for NaNs.  Made by :func:`checkpoint8` or
+    a step, ``amax / 254`` of its block's largest magnitude -- by up to a whole step in the checkpoint that :func:`group_norm_act` writes for ReLU or LeakyReLU,
+    where an element whose rounded value lies on the other side of the activation's border takes its other neighbour.  A block with a NaN or an infinity stands for NaNs.  Made by :func:`checkpoint8` or
     :func:`group_norm_act`; read by :func:`checkpoint8_restore`, :func:`group_norm_act_apply` and :func:`group_norm_act_bwd`."""
     __slots__ = ('q', 'scale', 'shape', 'dtype', 'device')
 

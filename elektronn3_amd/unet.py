@@ -1267,12 +1267,12 @@ class UNet(nn.Module):
     @torch.jit.unused
     def checkpoint8(self, enabled=True):
         """Keeps the activations of training forwards in 8 bits until their backward (about 1/7 of the memory of a pending graph; the forward and the backward
-        each need the full buffer while they run).  For several graphs that are alive at once: accumulation over networks or views, and
-        ``normalization='group'`` / ``'instance'``, whose batch is one graph per sample.  The outputs are unchanged; the gradients are those of the rounded
-        tensors: of every norm's input, an element is off by at most 1/254 of the largest of its block of 64 (:class:`elektronn3_amd.ops.Checkpoint8`),
-        and the activations are recomputed from them.  What the reference's ``forward_gradcp`` (unet.py:918-935) trades recomputation for, this trades
-        precision for.  The rounding keeps elements on their side of a ReLU's border, and a pooling window's maximum in place where a neighbouring code on that
-        side allows it (all but some 10 windows in a million).  fp32 compute; transposed
+        each need the full buffer while they run, so that the peak of a step with ONE graph at a time grows by that 1/7).  For several graphs that are alive at once:
+        accumulation over networks or views, and ``normalization='group'`` / ``'instance'``, whose batch is one graph per sample.  The outputs are unchanged; the
+        gradients are those of the rounded tensors: of every norm's input, an element is off by at most 1/254 of the largest of its block of 64
+        (:class:`elektronn3_amd.ops.Checkpoint8`), and the activations are recomputed from them.  The rounding keeps elements on their side of a ReLU's border, and a
+        pooling window's maximum in place where a neighbouring code on that side allows it (all but some 10 windows in a million); elements moved for that are off
+        by up to 1/127.  What the reference's ``forward_gradcp`` (unet.py:918-935) trades recomputation for, this trades precision for.  fp32 compute; transposed
         up-convolutions, 'same' convolutions and a norm behind every convolution, no attention (NotImplementedError otherwise).  Scripted modules keep
         their activations as they are.  Returns the module."""
         if enabled:

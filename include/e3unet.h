@@ -190,7 +190,7 @@ int e3_unet_backward_loss(e3_unet_plan* plan, void* stream, const float* y, cons
  * vectors into `kept` (e3_unet_checkpoint8_bytes() bytes, about 1/7 of `saved`), after which `saved` may be reused; _restore fills a `saved`
  * buffer for e3_unet_backward* of the same plan, shape and parameters, recomputing the activations from the restored tensors.  The gradients are
  * those of the rounded tensors; the rounding keeps elements on their side of a ReLU's border, and a pooling window's maximum in place where a neighbouring
- * code on that side allows it (all but some 10 windows in a million).
+ * code on that side allows it (all but some 10 windows in a million): an element is off by up to a step, 1/127 of the largest magnitude of its block.
  * nn.RReLU: e3_unet_set_rrelu with the forward's seed first.  fp32 path; 'same' convs, transposed convs and a norm behind every conv, no attention,
  * not the ResUNet (E3_ERR_UNSUPPORTED otherwise). */
 int e3_unet_checkpoint8_bytes(const e3_unet_plan* plan, int N, int D, int H, int W, size_t* kept_bytes);
@@ -284,7 +284,8 @@ int e3_bn_relu_bwd(void* stream, const float* x, int x_ldc, const float* mean, c
  *     y = act((x - mean) * rstd * gamma + beta),   rstd = (var + eps)^-1/2.
  *   gamma, beta: [C] fp32, or NULL (1 and 0).  act_slope: 0 = ReLU, (0, 1) = LeakyReLU, 1 = identity, 2 = SiLU.
  *   mean, rstd:  [N][G] fp32 outputs (inputs of _apply and _bwd).
- *   q, q_scale:  NULL, or the 8-bit checkpoint of x that the same call writes (see e3_checkpoint8_pack; N*D*H*W*C codes).
+ *   q, q_scale:  NULL, or the 8-bit checkpoint of x that the same call writes (see e3_checkpoint8_pack; N*D*H*W*C codes).  With ReLU or LeakyReLU (slope < 1) an
+ *                element whose rounded value lies on the other side of z = 0 takes the code of its other neighbour (clamped to +-127): off by up to a whole step there.
  *   workspace:   e3_group_norm_workspace_bytes(.., backward) bytes, 16-byte aligned; NULL where that is 0 (small groups need none).
  * y may be x itself (the same view), dx may be dy.  Statistics are fp32 values of fp64 sums; gradient sums add at most 512 elements in fp32, then in fp64; the
  * order is fixed, two identical calls give the same bits.  At most 2^23 - 1 groups in all samples and 2^26 channels (E3_ERR_UNSUPPORTED). */
