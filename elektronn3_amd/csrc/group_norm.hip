@@ -11,7 +11,7 @@
 // consecutive channels of a piece that surely share a group (8, 4 or 1): V / UN constants or sums per thread instead of V, which decides the register count.
 //   forward:   statistics (read x) -> apply (read x, write y [, write the checkpoint])
 //   backward:  reduce (read x, dy) -> apply (read x, dy, write dx)
-//   small groups: one launch each way, the pieces held in registers in between
+//   small groups: one launch each way, the pieces held in registers in between (the forward's not where too many groups share a line: map_group_fwd)
 // What bounds them: HBM, or the memory-side cache, for tensors above some 16 MB, where the second read of the inputs is the price of two passes; below, the latency of
 // two dependent launches (4 - 6 us each), and of the calling program.  2 x 64 x 128 x 128 x 32, 8 groups:
 //   fp32 forward 46 us (5.8 TB/s) + 83 (6.5), fp32 backward from a checkpoint 64 (5.3) + 97 (6.3), bf16 backward 51 (5.3) + 66 (6.1)
@@ -690,9 +690,11 @@ constexpr int SUM_TERMS = 512;               // fp32 terms of a sum: their round
 
 void set_shape(GnArgs& a, const Shape& sh) { a.N = sh.N; a.S = sh.S; a.C = sh.C; a.G = sh.G; a.cg = sh.C / sh.G; a.inv_m = 1.0 / ((double)sh.S * a.cg); }
 
-// Twice as many where a backward's workgroups have 16 steps or more and a sample's records stay few (2 x 64 x 128 x 128 x 32 in 8 groups: fp32 226 -> 213 us, from a checkpoint 182 -> 167,
-// bf16 from a checkpoint 120 -> 111, but not bf16 116 -> 122; one sample of half the size in 32 groups would lose 65 -> 73), or for rows of single elements, whose loads are small
-// (1 x 19 x 27 x 89 x 65: forward 24 -> 20 us; three workgroups per CU in its backward, from a checkpoint 26 -> 22)
+// Twice as many where a backward's workgroups have 16 steps or more and a sample's records stay few (us of a call in a replayed graph, two -> four workgroups per CU.  2 x 64 x 128 x 128 x 32 in 8 groups: fp32
+// 234 -> 219, from a checkpoint 169 -> 164, bf16 from a checkpoint 111 -> 106, but bf16 129 -> 131; 4 x 64 x 64 x 64 x 64 in 8: fp32 233 -> 218, bf16 from a checkpoint 123 -> 112; one sample
+// 64 x 128 x 128 x 32 in 32, bf16 from a checkpoint, would lose 65 -> 71), or for rows of single elements, whose loads are small (bf16 forward of 1 x 19 x 27 x 89 x 65 in 1 group 28 -> 22,
+// 1 x 41 x 64 x 65 x 33 in 3 41 -> 30, 2 x 30 x 100 x 101 x 7 in 7 31 -> 25; their backwards with two, three, four per CU: 23.3, 20.0, 20.2; 30.1, 25.5, 24.8; 24.8, 22.2, 22.5, and 20.2,
+// 18.3, 19.3 for 3 x 17 x 45 x 51 x 25 in 5)
 template <int V> int workgroups(const Shape& sh, bool backward, bool ck = true) {
     const long long steps = sh.N * sh.S * (sh.C / V) / (PASS_T * U2<V>);
     if (V == 1) return !backward ? 2 * PASS_WGS : steps >= 2 * PASS_WGS ? PASS_WGS * 3 / 2 : PASS_WGS;
@@ -758,7 +760,7 @@ template <int V> bool map_group(GnArgs& a, const Shape& sh) {
     return true;
 }
 // ... of the forward, for elements of `size` bytes.  A bundle narrower than a 128-byte line moves every line once per bundle in it, to as many workgroups on other XCDs: what that moves is
-// limited.  us for two launches : one, 16-bit types unless said, by megabytes moved so:
+// limited.  us of a call in a replayed graph, two launches : one, 16-bit types unless said, by megabytes moved so:
 //   pieces: 32: 14.3 : 12.8 (2 x 2048 voxels x 512 in 64 groups), 11.7 : 11.7 (16 x 2048 x 64 in 8), fp32 12.5 : 13.6 (4 x 4096 x 64 in 16); 40: 15.0 : 13.9 (5 x 2048 x 256 in 32);
 //     48: 13.4 : 16.6 (24 x 2048 x 64 in 8); 64: 17.5 : 19.6 (4 x 2048 x 512 in 64); 1024: 76 : 236 (64 of these)
 //   single elements instead of two launches with pieces: 16: 10.7 : 9.1 (2 x 4096 x 32 in 32); 21: 14.6 : 11.9 (16 x 105 x 1200 in 100); 31: 15.0 : 16.6 (300 x 105 x 96 in 8);
