@@ -367,7 +367,8 @@ def _chk_any(t, name, shape=None, dtype=None, device=None):
         raise ValueError(f'{name}: expected a 5D (N, D, H, W, C) tensor, got {t.dim()}D')
     if not t.is_contiguous():
         return _ldc(t)
-    return _rows(t.shape[4] or 1)
+    C = t.shape[4]
+    return C or 1 if C < 1 << 31 else _rows(C)
 
 
 def _span(t):
