@@ -177,3 +177,31 @@ def test_saved_activations(kw, shape, act):
         if t is not None:
             C = t.shape[-1]
             assert torch.equal(t, got.cat[j][..., :C] + got.cat[j][..., C:])
+
+
+@pytest.mark.parametrize('kw,shape,act', CASES[1:])
+def test_backward_reads_only_what_is_restored(monkeypatch, kw, shape, act):
+    """The gradients from buffers whose bytes were all NaN before the forward or the restoring filled them; and those of a full graph that is given the restored tensors."""
+    from elektronn3_amd import _lib, unet
+    torch.manual_seed(5)
+    kw = dict(kw)
+    m = unet.UNet(kw.pop('in_channels', 1), 2, **kw).cuda().train()
+    g = torch.Generator().manual_seed(9)
+    x, dy = torch.randn(shape, generator=g).cuda(), torch.randn(shape[0], 2, *shape[2:], generator=g).cuda()
+
+    def gradients(out):
+        m.zero_grad()
+        out.backward(dy)
+        return [p.grad.clone() for p in m.parameters()]
+    m.checkpoint8()
+    want = gradients(forward(m, x, 11)[0])
+    monkeypatch.setattr(unet, '_alloc_saved', lambda device, n: torch.full((int(n),), 255, dtype=torch.uint8, device=device))
+    got = gradients(forward(m, x, 11)[0])
+    assert all(bool(torch.isfinite(p).all()) and torch.equal(p, q) for p, q in zip(got, want))
+    out8, node8 = forward(m, x, 11)
+    m.checkpoint8(False)
+    out, node = forward(m, x, 11)
+    if node8.rrelu is not None:
+        _lib.check(_lib.load().e3_unet_set_rrelu(m._plan().handle, *node8.rrelu))
+    node.saved_buf = node8.saved_buf.restore(node8.tens.tens)
+    assert all(torch.equal(p, q) for p, q in zip(gradients(out), want))
