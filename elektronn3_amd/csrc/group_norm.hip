@@ -760,11 +760,13 @@ template <int V> bool map_group(GnArgs& a, const Shape& sh) {
     return true;
 }
 // ... of the forward, for elements of `size` bytes.  A bundle narrower than a 128-byte line moves every line once per bundle in it, to as many workgroups on other XCDs: what that moves is
-// limited.  us of a call in a replayed graph, two launches : one, 16-bit types unless said, by megabytes moved so:
+// limited.  us of a call in a replayed graph, two launches : one, 16-bit types unless said, by megabytes moved so (two launches and their workspace cost an eager call 4 us of the host's time
+// besides, which shows where the GPU takes less than some 15 us: 15.5 : 14.6 for 24 x 2048 x 64, 15.5 : 11.6 for 2 x 4096 x 64, but 17.0 : 17.7 for 4 x 2048 x 512):
 //   pieces: 32: 14.3 : 12.8 (2 x 2048 voxels x 512 in 64 groups), 11.7 : 11.7 (16 x 2048 x 64 in 8), fp32 12.5 : 13.6 (4 x 4096 x 64 in 16); 40: 15.0 : 13.9 (5 x 2048 x 256 in 32);
 //     48: 13.4 : 16.6 (24 x 2048 x 64 in 8); 64: 17.5 : 19.6 (4 x 2048 x 512 in 64); 1024: 76 : 236 (64 of these)
 //   single elements instead of two launches with pieces: 16: 10.7 : 9.1 (2 x 4096 x 32 in 32); 21: 14.6 : 11.9 (16 x 105 x 1200 in 100); 31: 15.0 : 16.6 (300 x 105 x 96 in 8);
-//     32: 11.2 : 10.7, with a checkpoint 13.0 : 17.5 (1 x 4096 x 64 in 64); 41: 15.8 : 21.4 (32 x 105 x 1200 in 100); 1024: 34 : 88 (8 x 4096 x 256 in 256)
+//     41: 15.8 : 21.4 (32 x 105 x 1200 in 100); one-channel groups 32: 11.2 : 10.7 (1 x 4096 x 64 in 64); 64: 11.4 : 12.1 (2 x 4096 x 64 in 64); 256: 16.1 : 24.3 (4 x 4096 x 128 in 128);
+//     1024: 34 : 88 (8 x 4096 x 256 in 256)
 //   single elements in either form: 5 bundles to a line 385: 130 : 113 (400 x 315 x 300 in 25); 21 and 33 of them 41: 15.0 : 10.9 (16 x 315 x 201 in 67), 12.6 : 12.2 (64 x 315 x 33 in 33),
 //     165: 26 : 31, 18 : 33 (four times these)
 // Bundles of whole lines have no limit (1024 x 256 x 512 in 8: 150 : 142).
@@ -772,7 +774,9 @@ template <int V> bool map_group_fwd(GnArgs& a, const Shape& sh, int size, bool r
     if (!map_group<V>(a, sh)) return false;
     const long long row = (long long)sh.C * size, width = (long long)a.PT * V * size, line = row < 128 ? row : 128;
     if (width >= line || (!rows_of_pieces && line <= 8 * width)) return true;
-    return sh.N * sh.S * (row / width) * line <= (V > 1 ? 40ll : rows_of_pieces ? 24ll : 96ll) << 20;
+    const int piece = 16 / size;
+    const bool cut = a.cg % piece != 0 && piece % a.cg != 0;
+    return sh.N * sh.S * (row / width) * line <= (V > 1 ? 48ll : !rows_of_pieces ? 96ll : cut ? 32ll : 64ll) << 20;
 }
 // ... and of the backward, whose workgroups walk the samples: 6 us for the first and 3 - 9 for each other one (a workgroup's 16-byte pieces lie C elements apart) against
 // 9 - 13 for two launches, which cost the host 5 us more.  1 x 4 x 8 x 8 x 128 in 8 groups, fp16: 8.4 us instead of 12.2, eagerly 13 instead of 18; two samples of it 14.2

@@ -22,7 +22,7 @@ def test_forwards_in_two_launches(dims):
 
 
 @pytest.mark.parametrize('dims', [
-    (1, 4, 8, 8, 128, 8), (4, 1, 5, 7, 24, 3), (1, 16, 16, 16, 8, 8), (16, 3, 5, 7, 1200, 100), (64, 8, 8, 8, 64, 8), (100, 5, 7, 9, 60, 5),
+    (1, 4, 8, 8, 128, 8), (4, 1, 5, 7, 24, 3), (1, 16, 16, 16, 8, 8), (1, 16, 16, 16, 64, 64), (16, 3, 5, 7, 1200, 100), (64, 8, 8, 8, 64, 8), (100, 5, 7, 9, 60, 5),
     (1024, 1, 7, 9, 512, 8),        # whole lines: no limit
 ])
 def test_forwards_in_one_launch(dims):
